@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define NQ_ABI_VERSION 7
+#define NQ_ABI_VERSION 8
 
 /* status codes */
 #define NQ_OK 0
@@ -57,6 +57,9 @@ extern "C" {
 #define NQ_FMT_W4_GROUP 2    /* uint4, 2 per byte (low nibble = even k), fp16
                                 scale and uint4 zero-point per group along IN */
 #define NQ_FMT_FP8_E4M3 3    /* OCP e4m3fn [OUT, IN] + one fp32 scale */
+#define NQ_FMT_FP8_BLOCK 4   /* OCP e4m3fn [OUT, IN] + one fp32 scale per block
+                                of 128 x 128; x as e4m3fn codes with one fp32
+                                scale per row and 128 of IN */
 
 /* element types of x, y, bias */
 #define NQ_DT_F32 0
@@ -77,6 +80,8 @@ extern "C" {
                                   2 .. 512 activation rows, any width; int8 layers: 2 .. 16 rows up to IN = 4096),
                                   not only where they were measured to win: for tuning on other shapes, and for
                                   tests that walk every instantiation */
+#define NQ_FLAG_GRAD 4         /* FP8_BLOCK layers only: keep a second copy of the codes, of W^T, which
+                                  nq_grad_input_fp8_block reads (1 byte per weight) */
 
 /* epilogues (LinearAct's, noeira/nn/primitives/linear_act.mojo:81-115) */
 #define NQ_EPI_NONE 0
@@ -130,6 +135,12 @@ int32_t nq_set_weight_w4g(nq_handle h, const uint8_t* codes_host, const uint16_t
 /* NQ_FMT_FP8_E4M3: e4m3fn codes [OUT, IN] and the per-tensor scale. */
 int32_t nq_set_weight_fp8(nq_handle h, const uint8_t* w_host, float scale, void* stream);
 
+/* NQ_FMT_FP8_BLOCK: e4m3fn codes [OUT, IN] and scales [ceil(OUT/128), ceil(IN/128)] fp32, from the host or, with
+ * _dev, from device memory (a copy is made, in the matrix core's operand order; no logical bytes are kept for
+ * nq_get_blocks then).  Both return after the layer is ready. */
+int32_t nq_set_weight_fp8_block(nq_handle h, const uint8_t* codes_host, const float* scales_host, void* stream);
+int32_t nq_set_weight_fp8_block_dev(nq_handle h, const uint8_t* codes, const float* scales, void* stream);
+
 /* Bytes of the logical weight (`QLinear.BYTES`, qlinear.mojo:216-217, for
  * Q4_0; the codes' byte count for the other formats). */
 int64_t nq_blocks_bytes(nq_handle h);
@@ -157,7 +168,9 @@ int64_t nq_device_bytes(nq_handle h);
  *     y[M, OUT] = epi( x[M, IN] @ deq(W)^T  (+ bias[OUT]) )
  * x_dtype: F32 or BF16 for Q4_0 / W8_CHANNEL / W4_GROUP; I8 for W8_CHANNEL
  * (x_scale = fp32 [M], one per row); FP8_E4M3 for FP8_E4M3 weights
- * (x_scale = fp32 [1]).  x_scale is NULL otherwise.
+ * (x_scale = fp32 [1]) or FP8_BLOCK weights, which take nothing else (x_scale =
+ * fp32 [M, ceil(IN/128)], one per row and block: nq_quantize_rows_fp8_block).
+ * x_scale is NULL otherwise.
  * y_dtype: F32 or BF16; I32 with x_dtype I8 returns the raw accumulators
  * (no scale, bias or epilogue).  bias may be NULL; bias_dtype F32 or BF16.
  * The dequantised weight is never materialised.
@@ -176,7 +189,8 @@ int32_t nq_forward(nq_handle h, const void* x, int32_t x_dtype, const float* x_s
                    int32_t epilogue, void* stream);
 
 /* One layer made of the rows of up to four loaded layers that share their
- * input (same format, IN, group width; FP8_E4M3: same scale), e.g. q|k|v or
+ * input (same format, IN, group width; FP8_E4M3: same scale; FP8_BLOCK: all
+ * but the last a multiple of 128 rows, so that no two share a scale), e.g. q|k|v or
  * gate|up of a decoder layer: the seven projections the reference's caller
  * launches one by one (`DecoderLayerWeights.proj_fwd`,
  * noeira/deep_agents/smolvla/layer_weights.mojo:455-508, called from
@@ -248,6 +262,44 @@ int32_t nq_cast_pad_bf16(const float* src, uint16_t* dst, int32_t rows, int32_t 
  * [rows, cols]. */
 int32_t nq_slice_cast_f32(const uint16_t* src, float* dst, int32_t rows, int32_t cols,
                           int32_t cols_pad, void* stream);
+
+/* The activations of an FP8_BLOCK layer: x [M, K] -> e4m3fn codes [M, K] and scales [M, ceil(K/128)] fp32, for each
+ * row and block of 128 of K (the last one as wide as is left)
+ *     s = absmax / 448 (1 where the block is zero, never below 2^-126);  q = e4m3(clip(x / s, -448, 448))
+ * divisions as IEEE rounds them, codes to nearest, ties to even.  A block that holds a NaN or an infinity gets the scale
+ * NaN and codes 0x7F: all its values are NaN.  x F32 or BF16, any K >= 1; x and codes 16-byte aligned. */
+int32_t nq_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* codes, float* scales, int32_t M, int32_t K,
+                                   void* stream);
+
+/* The input gradient of an FP8_BLOCK layer made with NQ_FLAG_GRAD (`QLinear.vjp`, qlinear.mojo:479-518, with the
+ * gradient quantised as the activations are):
+ *     gx[M, IN] = gy[M, OUT] @ deq(W),   overwriting gx (F32 or BF16)
+ * gy: e4m3fn codes [M, OUT] with scales [M, ceil(OUT/128)] (nq_quantize_rows_fp8_block over OUT).  OUT must be a multiple
+ * of 16.  NQ_ERR_UNSUPPORTED for a layer made without the flag, and for one made by nq_fuse_rows (which keeps no W^T). */
+int32_t nq_grad_input_fp8_block(nq_handle h, const uint8_t* gy, const float* gy_scale, void* gx, int32_t gx_dtype,
+                                int32_t M, void* stream);
+
+/* Layer norm over rows of D values, y[M, D] = (x - mean) * rstd * gamma + beta with rstd = 1 / sqrt(var + eps), the
+ * variance divided by D; statistics in fp32.  x and y F32 or BF16 (y may be x where the types agree; otherwise they do
+ * not overlap); gamma, beta fp32 [D], or NULL for 1 and 0; mean, rstd fp32 [M] for the gradient, or both NULL.
+ * The _fp8_block form writes y as nq_quantize_rows_fp8_block would (codes [M, D], scales [M, ceil(D/128)]) from the fp32
+ * result, which is never stored: the norm in front of an FP8_BLOCK projection in one launch. */
+int32_t nq_layer_norm(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps, void* y,
+                      int32_t y_dtype, float* mean, float* rstd, int32_t M, int32_t D, void* stream);
+int32_t nq_layer_norm_fp8_block(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps,
+                                uint8_t* codes, float* scales, float* mean, float* rstd, int32_t M, int32_t D, void* stream);
+
+/* The gradients of nq_layer_norm from its input, its saved statistics and gy[M, D]:
+ *     a = gy * gamma, xh = (x - mean) * rstd
+ *     gx = rstd * (a - mean_D(a) - xh * mean_D(a * xh)),  dgamma = sum_M gy * xh,  dbeta = sum_M gy
+ * gx [M, D] F32 or BF16 (gx may be gy, or x, where the types agree); dgamma, dbeta fp32 [D] are overwritten (zeros for
+ * M = 0), or both NULL: no sums over the rows.  Their partial sums lie in `workspace` (16-byte aligned, at least
+ * nq_layer_norm_grad_workspace_bytes(M, D)), which holds nothing between calls; two calls that may run at once need
+ * one each.  The rows are added in a fixed order: the same inputs give the same bits. */
+int64_t nq_layer_norm_grad_workspace_bytes(int32_t M, int32_t D);
+int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, const float* rstd, const float* gamma,
+                           const void* gy, int32_t gy_dtype, void* gx, int32_t gx_dtype, float* dgamma, float* dbeta,
+                           int32_t M, int32_t D, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Three W8_CHANNEL layers run as one launch for batched-env actor inference
  * (SAC/PPO actor MLP; `LinearAct` chain): per token

@@ -7,13 +7,18 @@ libnoeira_qlinear.so is missing (there is no CPU path).
 """
 from ._lib import NQError  # noqa: F401
 
-__all__ = ["NQError", "QLinear", "W8Linear", "W4GroupLinear", "FP8Linear", "FusedRows"]
+__all__ = ["NQError", "QLinear", "W8Linear", "W4GroupLinear", "FP8Linear", "FP8BlockLinear", "FusedRows", "LayerNorm"]
 
 
 def __getattr__(name):
-    if name in ("QLinear", "W8Linear", "W4GroupLinear", "FP8Linear", "quantize_rows_i8",
+    if name in ("QLinear", "W8Linear", "W4GroupLinear", "FP8Linear", "FP8BlockLinear", "quantize_rows_i8",
+                "quantize_rows_fp8_block",
                 "cast_pad_bf16", "slice_cast_f32", "mlp3_w8a8_forward", "FusedRows"):
         from . import qlinear
 
         return getattr(qlinear, name)
+    if name == "LayerNorm":
+        from .norm import LayerNorm
+
+        return LayerNorm
     raise AttributeError(name)

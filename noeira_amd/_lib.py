@@ -15,13 +15,14 @@ LIB_NAME = "libnoeira_qlinear.so"
 
 # status codes / enums of include/noeira_qlinear.h
 NQ_OK, NQ_ERR_INVALID, NQ_ERR_NOT_LOADED, NQ_ERR_NO_BLOCKS, NQ_ERR_SIZE, NQ_ERR_HIP, NQ_ERR_UNSUPPORTED = range(7)
-FMT_Q4_0, FMT_W8_CHANNEL, FMT_W4_GROUP, FMT_FP8_E4M3 = range(4)
+FMT_Q4_0, FMT_W8_CHANNEL, FMT_W4_GROUP, FMT_FP8_E4M3, FMT_FP8_BLOCK = range(5)
 DT_F32, DT_BF16, DT_I8, DT_FP8_E4M3, DT_I32 = range(5)
 EPI_NONE, EPI_RELU, EPI_SWIGLU = 0, 1, 2
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 FLAG_NO_TILE_COPY = 1
 FLAG_PREFER_TILE = 2
+FLAG_GRAD = 4
 
 
 class LoraPart(C.Structure):
@@ -35,7 +36,10 @@ EXPORTS = [
     "nq_keep_only_repacked", "nq_device_bytes", "nq_workspace_bytes", "nq_set_workspace", "nq_forward", "nq_dequantize", "nq_grad_input", "nq_quantize_rows_i8",
     "nq_cast_pad_bf16", "nq_slice_cast_f32", "nq_mlp3_w8a8_forward", "nq_fuse_rows", "nq_fused_parts",
     "nq_forward_fused", "nq_fuse_glu", "nq_hessian_create", "nq_hessian_destroy", "nq_hessian_add", "nq_hessian_rows",
-    "nq_hessian_get", "nq_hessian_set", "nq_hinv_upper_f64", "nq_hinv_upper_f64_dev", "nq_set_weight_gptq", "nq_q4_0_objective", "nq_lora_forward_add", "nq_forward_lora", "nq_forward_fused_lora", "nq_diag_mfma_rate", "nq_diag_stream_read", "nq_diag_gemm8_timeline", "nq_diag_forward_a16", "nq_diag_forward_gemm8",
+    "nq_hessian_get", "nq_hessian_set", "nq_hinv_upper_f64", "nq_hinv_upper_f64_dev", "nq_set_weight_gptq", "nq_q4_0_objective", "nq_lora_forward_add", "nq_forward_lora", "nq_forward_fused_lora",
+    "nq_set_weight_fp8_block", "nq_set_weight_fp8_block_dev", "nq_quantize_rows_fp8_block", "nq_grad_input_fp8_block",
+    "nq_layer_norm", "nq_layer_norm_fp8_block", "nq_layer_norm_grad", "nq_layer_norm_grad_workspace_bytes",
+    "nq_diag_mfma_rate", "nq_diag_stream_read", "nq_diag_gemm8_timeline", "nq_diag_forward_a16", "nq_diag_forward_gemm8",
 ]
 
 
@@ -174,6 +178,22 @@ def lib() -> C.CDLL:
     L.nq_set_workspace.argtypes = [p, p, i64]
     L.nq_diag_forward_a16.restype = i32
     L.nq_diag_forward_a16.argtypes = [p, p, i32, p, i32, i32, i32, i32, p]
+    L.nq_set_weight_fp8_block.restype = i32
+    L.nq_set_weight_fp8_block.argtypes = [p, p, p, p]
+    L.nq_set_weight_fp8_block_dev.restype = i32
+    L.nq_set_weight_fp8_block_dev.argtypes = [p, p, p, p]
+    L.nq_quantize_rows_fp8_block.restype = i32
+    L.nq_quantize_rows_fp8_block.argtypes = [p, i32, p, p, i32, i32, p]
+    L.nq_grad_input_fp8_block.restype = i32
+    L.nq_grad_input_fp8_block.argtypes = [p, p, p, p, i32, i32, p]
+    L.nq_layer_norm.restype = i32
+    L.nq_layer_norm.argtypes = [p, i32, p, p, f32, p, i32, p, p, i32, i32, p]
+    L.nq_layer_norm_fp8_block.restype = i32
+    L.nq_layer_norm_fp8_block.argtypes = [p, i32, p, p, f32, p, p, p, p, i32, i32, p]
+    L.nq_layer_norm_grad_workspace_bytes.restype = i64
+    L.nq_layer_norm_grad_workspace_bytes.argtypes = [i32, i32]
+    L.nq_layer_norm_grad.restype = i32
+    L.nq_layer_norm_grad.argtypes = [p, i32, p, p, p, p, i32, p, i32, p, p, i32, i32, p, i64, p]
     got = L.nq_abi_version()
     if got != ABI_VERSION:
         raise OSError(f"{LIB_NAME}: ABI version {got}, this package binds version {ABI_VERSION}")

@@ -42,6 +42,7 @@ const char* fmt_name(int f) {
         case NQ_FMT_W8_CHANNEL: return "W8_CHANNEL";
         case NQ_FMT_W4_GROUP: return "W4_GROUP";
         case NQ_FMT_FP8_E4M3: return "FP8_E4M3";
+        case NQ_FMT_FP8_BLOCK: return "FP8_BLOCK";
     }
     return "?";
 }
@@ -65,6 +66,9 @@ void free_device(nq_layer* L) {
     if (L->d_tiled) (void)hipFree(L->d_tiled);
     if (L->d_tile16) (void)hipFree(L->d_tile16);
     if (L->d_tile16_scales) (void)hipFree(L->d_tile16_scales);
+    if (L->d_codes_t) (void)hipFree(L->d_codes_t);
+    if (L->d_scales_t) (void)hipFree(L->d_scales_t);
+    L->d_codes_t = nullptr, L->d_scales_t = nullptr;
     L->d_codes = nullptr, L->d_scales = nullptr, L->d_zps = nullptr, L->d_tiled = nullptr;
     L->d_tile16 = nullptr, L->d_tile16_scales = nullptr, L->tile_nj = 0, L->tiled_bytes = 0;
 }
@@ -137,11 +141,16 @@ int32_t nq_create(nq_handle* out, int32_t format, int32_t in_features, int32_t o
                   int32_t flags) {
     if (!out) return fail(NQ_ERR_INVALID, "nq_create: null output handle");
     *out = nullptr;
-    if (format < NQ_FMT_Q4_0 || format > NQ_FMT_FP8_E4M3)
+    if (format < NQ_FMT_Q4_0 || format > NQ_FMT_FP8_BLOCK)
         return fail(NQ_ERR_INVALID, "nq_create: unknown format " + std::to_string(format));
     if (in_features <= 0 || out_features <= 0)
         return fail(NQ_ERR_INVALID, "nq_create: IN and OUT must be positive");
-    if (flags & ~(NQ_FLAG_NO_TILE_COPY | NQ_FLAG_PREFER_TILE)) return fail(NQ_ERR_INVALID, "nq_create: unknown flags");
+    if (flags & ~(NQ_FLAG_NO_TILE_COPY | NQ_FLAG_PREFER_TILE | NQ_FLAG_GRAD)) return fail(NQ_ERR_INVALID, "nq_create: unknown flags");
+    if (flags & NQ_FLAG_GRAD) {
+        if (format != NQ_FMT_FP8_BLOCK) return fail(NQ_ERR_INVALID, "nq_create: NQ_FLAG_GRAD is for FP8_BLOCK layers");
+        if (out_features % 16 != 0)
+            return fail(NQ_ERR_INVALID, "nq_create: NQ_FLAG_GRAD needs OUT to be a multiple of 16");
+    }
     if (format == NQ_FMT_Q4_0) {
         // qlinear.mojo:243-245
         if (in_features % Q4_GROUP != 0)
@@ -158,14 +167,15 @@ int32_t nq_create(nq_handle* out, int32_t format, int32_t in_features, int32_t o
         if (in_features % 16 != 0)
             return fail(NQ_ERR_INVALID, std::string("nq_create: ") + fmt_name(format) +
                                             " needs IN to be a multiple of 16");
-        group = 0;
+        group = format == NQ_FMT_FP8_BLOCK ? FP8_BLOCK : 0;
     }
     nq_layer* L = new (std::nothrow) nq_layer();
     if (!L) return fail(NQ_ERR_INVALID, "nq_create: out of host memory");
     L->format = format, L->in = in_features, L->out = out_features, L->group = group;
-    L->groups = group ? (in_features + group - 1) / group : 0;
+    L->groups = group ? (in_features - 1) / group + 1 : 0;
     L->no_tile_copy = (flags & NQ_FLAG_NO_TILE_COPY) != 0;
     L->prefer_tile = (flags & NQ_FLAG_PREFER_TILE) != 0;
+    L->keep_grad = (flags & NQ_FLAG_GRAD) != 0;
     *out = L;
     return NQ_OK;
 }
@@ -355,6 +365,72 @@ int32_t nq_set_weight_fp8(nq_handle h, const uint8_t* w_host, float scale, void*
     return NQ_OK;
 }
 
+// the layer's arrays from row-ordered codes and scales on the device
+static int32_t adopt_fp8_block(nq_layer* L, const uint8_t* codes, const float* scales, hipStream_t s) {
+    const int64_t G = L->groups, NB = ((int64_t)L->out + FP8_BLOCK - 1) / FP8_BLOCK;
+    NQ_HIP(hipMalloc((void**)&L->d_codes, (size_t)(((int64_t)L->out + 15) / 16 * G * 2048)));
+    NQ_HIP(hipMalloc(&L->d_scales, (size_t)(NB * G) * 4));
+    int32_t rc = launch_fp8_block_repack(codes, L->d_codes, L->out, L->in, false, s);
+    if (rc) return rc;
+    NQ_HIP(hipMemcpyAsync(L->d_scales, scales, (size_t)(NB * G) * 4, hipMemcpyDeviceToDevice, s));
+    if (L->keep_grad) {
+        NQ_HIP(hipMalloc((void**)&L->d_codes_t, (size_t)(((int64_t)L->in + 15) / 16 * NB * 2048)));
+        NQ_HIP(hipMalloc((void**)&L->d_scales_t, (size_t)(NB * G) * 4));
+        if ((rc = launch_fp8_block_repack(codes, L->d_codes_t, L->out, L->in, true, s))) return rc;
+        if ((rc = launch_fp8_block_scales_t(scales, L->d_scales_t, (int32_t)NB, (int32_t)G, s))) return rc;
+    }
+    L->row_bytes = G * FP8_BLOCK;
+    NQ_HIP(hipStreamSynchronize(s));
+    return NQ_OK;
+}
+
+static int32_t set_weight_fp8_block(nq_handle h, const uint8_t* codes, const float* scales, bool host, void* stream) {
+    int32_t rc = check_handle(h, "nq_set_weight_fp8_block");
+    if (rc) return rc;
+    if (h->format != NQ_FMT_FP8_BLOCK)
+        return fail(NQ_ERR_INVALID, "nq_set_weight_fp8_block: the layer's format is not FP8_BLOCK");
+    if (!codes || !scales) return fail(NQ_ERR_INVALID, "nq_set_weight_fp8_block: null codes or scales");
+    hipStream_t s = (hipStream_t)stream;
+    h->loaded = false;
+    if ((rc = bind_device(h))) return rc;
+    free_device(h);
+    const size_t n = (size_t)h->in * h->out;
+    const size_t ns = (((size_t)h->out + FP8_BLOCK - 1) / FP8_BLOCK) * (size_t)h->groups;
+    h->has_host_blocks = host;
+    std::vector<uint8_t>().swap(h->host_blocks);
+    if (host) {
+        try {
+            h->host_blocks.assign(codes, codes + n);
+        } catch (const std::bad_alloc&) {
+            return fail(NQ_ERR_INVALID, "nq_set_weight_fp8_block: out of host memory");
+        }
+        uint8_t* raw = nullptr;  // the codes, and behind them the scales
+        const size_t at = (n + 255) / 256 * 256;
+        hipError_t e = hipMalloc((void**)&raw, at + ns * 4);
+        if (e == hipSuccess) e = hipMemcpyAsync(raw, codes, n, hipMemcpyHostToDevice, s);
+        if (e == hipSuccess) e = hipMemcpyAsync(raw + at, scales, ns * 4, hipMemcpyHostToDevice, s);
+        if (e == hipSuccess) rc = adopt_fp8_block(h, raw, reinterpret_cast<const float*>(raw + at), s);
+        (void)hipFree(raw);
+        if (e != hipSuccess) rc = fail_hip(e, "nq_set_weight_fp8_block upload");
+    } else {
+        rc = adopt_fp8_block(h, codes, scales, s);
+    }
+    if (rc) {
+        free_device(h);
+        return rc;
+    }
+    h->loaded = true;
+    return NQ_OK;
+}
+
+int32_t nq_set_weight_fp8_block(nq_handle h, const uint8_t* codes_host, const float* scales_host, void* stream) {
+    return set_weight_fp8_block(h, codes_host, scales_host, true, stream);
+}
+
+int32_t nq_set_weight_fp8_block_dev(nq_handle h, const uint8_t* codes, const float* scales, void* stream) {
+    return set_weight_fp8_block(h, codes, scales, false, stream);
+}
+
 int64_t nq_blocks_bytes(nq_handle h) {
     if (!h) return 0;
     return logical_bytes(h);
@@ -380,6 +456,12 @@ int64_t nq_device_bytes(nq_handle h) {
         case NQ_FMT_Q4_0: n += rows * (h->in / Q4_GROUP) * 2; break;
         case NQ_FMT_W4_GROUP: n += rows * h->groups * 3; break;  // fp16 scale + one byte of zero point per group
         case NQ_FMT_W8_CHANNEL: n += rows * 4; break;
+        case NQ_FMT_FP8_BLOCK: {
+            const int64_t nb = (rows + FP8_BLOCK - 1) / FP8_BLOCK;
+            n = (rows + 15) / 16 * h->groups * 2048 + nb * h->groups * 4;
+            if (h->d_codes_t) n += ((int64_t)h->in + 15) / 16 * nb * 2048 + nb * h->groups * 4;
+            break;
+        }
         default: break;
     }
     if (h->d_tiled) n += h->tiled_bytes;
@@ -417,6 +499,8 @@ void row_view(const nq_layer* L, int r0, int r1, nq_layer* v) {
         default: srow = 0;
     }
     v->d_scales = L->d_scales ? reinterpret_cast<uint8_t*>(L->d_scales) + r0 * srow : nullptr;
+    if (L->format == NQ_FMT_FP8_BLOCK)  // (parts begin on a multiple of 128 rows: nq_fuse_rows)
+        v->d_scales = reinterpret_cast<float*>(L->d_scales) + (int64_t)(r0 / FP8_BLOCK) * L->groups;
     // the tile-ordered copy is in units of 16 rows: a part that starts on one has its own view of it
     v->prefer_tile = L->prefer_tile, v->no_tile_copy = L->no_tile_copy;
     if (L->d_tile16 && r0 % 16 == 0) {
@@ -438,6 +522,7 @@ int32_t dispatch(const ForwardArgs& a) {
                                             ", M = " + std::to_string(a.M) + "): run gate | up with nq_forward_fused "
                                             "and apply SwiGLU separately");
     }
+    if (a.L->format == NQ_FMT_FP8_BLOCK) return launch_fp8_block(a);
     if (a.x_dtype == NQ_DT_I8) {
         if (tile8_i8_applicable(a)) return launch_tile8_i8(a);
         if (gemm8_applicable(a)) return launch_gemm8(a);
@@ -459,6 +544,7 @@ int32_t dispatch(const ForwardArgs& a) {
 
 // the kernels that place rows through the part table themselves (one launch for all parts)
 bool places_parts(const ForwardArgs& a) {
+    if (a.L->format == NQ_FMT_FP8_BLOCK) return true;
     if (a.x_dtype == NQ_DT_I8) return false;
     if (gemv_fp8_applicable(a) || gemm8_applicable(a)) return false;
     if (gemm_tile_mt_splits_parts(a)) return false;  // wide and narrow parts: each on the kernel of its own layer
@@ -511,11 +597,16 @@ int32_t forward_impl(nq_handle h, const void* x, int32_t x_dtype, const float* x
         if (y_dtype != NQ_DT_F32 && y_dtype != NQ_DT_BF16)
             return fail(NQ_ERR_INVALID, "nq_forward: y must be fp32 or bf16");
         if (x_dtype == NQ_DT_FP8_E4M3) {
-            if (h->format != NQ_FMT_FP8_E4M3)
+            if (h->format != NQ_FMT_FP8_E4M3 && h->format != NQ_FMT_FP8_BLOCK)
                 return fail(NQ_ERR_INVALID, "nq_forward: fp8 activations need an FP8_E4M3 layer");
             if (!x_scale) return fail(NQ_ERR_INVALID, "nq_forward: fp8 activations need a scale");
+            if (h->format == NQ_FMT_FP8_BLOCK && ((uintptr_t)x_scale & 3))
+                return fail(NQ_ERR_INVALID, "nq_forward: x_scale must be 4-byte aligned");
         } else if (x_dtype != NQ_DT_F32 && x_dtype != NQ_DT_BF16) {
             return fail(NQ_ERR_INVALID, "nq_forward: unknown x dtype " + std::to_string(x_dtype));
+        } else if (h->format == NQ_FMT_FP8_BLOCK) {
+            return fail(NQ_ERR_INVALID, "nq_forward: an FP8_BLOCK layer takes e4m3 codes with block scales "
+                                        "(nq_quantize_rows_fp8_block)");
         }
     }
     ForwardArgs a{h, x, x_dtype, x_scale, seg.y[0], y_dtype, M, bias, bias_dtype, epilogue, (hipStream_t)stream, seg};
@@ -591,6 +682,8 @@ int32_t nq_fuse_rows(nq_handle* out, const nq_handle* layers, int32_t n, void* s
         if (a->format == NQ_FMT_FP8_E4M3 && b->scale != a->scale)
             return fail(NQ_ERR_INVALID, "nq_fuse_rows: FP8_E4M3 layers must share their per-tensor scale");
         if (!b->seg_end.empty() || b->glu) return fail(NQ_ERR_INVALID, "nq_fuse_rows: a fused layer cannot be fused again");
+        if (a->format == NQ_FMT_FP8_BLOCK && i + 1 < n && b->out % FP8_BLOCK != 0)
+            return fail(NQ_ERR_INVALID, "nq_fuse_rows: FP8_BLOCK layers but the last must have a multiple of 128 rows");
         rows += b->out;
     }
     if (rows > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_fuse_rows: too many rows");
@@ -613,6 +706,45 @@ int32_t nq_fuse_rows(nq_handle* out, const nq_handle* layers, int32_t n, void* s
         default: scale_row = 0;
     }
     hipStream_t s = (hipStream_t)stream;
+    if (a->format == NQ_FMT_FP8_BLOCK) {
+        // whole tiles of 16 rows and whole rows of block scales one behind the other
+        const int64_t srow = (int64_t)a->groups * 4;
+        hipError_t e = hipMalloc((void**)&F->d_codes, (size_t)((rows + 15) / 16 * 16 * F->row_bytes));
+        if (e == hipSuccess) e = hipMalloc(&F->d_scales, (size_t)((rows + FP8_BLOCK - 1) / FP8_BLOCK * srow));
+        int64_t r0 = 0;
+        bool all_blocks = true;
+        for (int i = 0; i < n && e == hipSuccess; i++) {
+            const nq_layer* b = layers[i];
+            e = hipMemcpyAsync(F->d_codes + r0 * F->row_bytes, b->d_codes, (size_t)(((int64_t)b->out + 15) / 16 * 16 * F->row_bytes),
+                               hipMemcpyDeviceToDevice, s);
+            if (e == hipSuccess)
+                e = hipMemcpyAsync(reinterpret_cast<uint8_t*>(F->d_scales) + r0 / FP8_BLOCK * srow, b->d_scales,
+                                   (size_t)(((int64_t)b->out + FP8_BLOCK - 1) / FP8_BLOCK * srow), hipMemcpyDeviceToDevice, s);
+            r0 += b->out;
+            F->seg_end.push_back((int32_t)r0);
+            all_blocks = all_blocks && b->has_host_blocks;
+        }
+        if (e == hipSuccess) e = hipStreamSynchronize(s);
+        if (e != hipSuccess) {
+            free_device(F);
+            delete F;
+            return fail_hip(e, "nq_fuse_rows");
+        }
+        if (all_blocks) {
+            try {
+                for (int i = 0; i < n; i++)
+                    F->host_blocks.insert(F->host_blocks.end(), layers[i]->host_blocks.begin(), layers[i]->host_blocks.end());
+            } catch (const std::bad_alloc&) {
+                free_device(F);
+                delete F;
+                return fail(NQ_ERR_INVALID, "nq_fuse_rows: out of host memory");
+            }
+            F->has_host_blocks = true;
+        }
+        F->loaded = true;
+        *out = F;
+        return NQ_OK;
+    }
     hipError_t e = hipMalloc((void**)&F->d_codes, (size_t)(rows * F->row_bytes) + 128);
     if (e == hipSuccess && scale_row) e = hipMalloc(&F->d_scales, (size_t)(rows * scale_row) + 128);
     if (e == hipSuccess && a->d_zps) e = hipMalloc((void**)&F->d_zps, (size_t)(rows * F->groups) + 128);
@@ -664,7 +796,7 @@ int32_t nq_fuse_glu(nq_handle* out, nq_handle gate, nq_handle up, void* stream) 
     }
     const nq_layer* a = gate;
     const nq_layer* b = up;
-    if (a->format == NQ_FMT_FP8_E4M3)
+    if (a->format == NQ_FMT_FP8_E4M3 || a->format == NQ_FMT_FP8_BLOCK)
         return fail(NQ_ERR_UNSUPPORTED, "nq_fuse_glu: Q4_0, W4_GROUP and W8_CHANNEL layers only");
     if (b->format != a->format || b->in != a->in || b->out != a->out || b->group != a->group || b->device != a->device)
         return fail(NQ_ERR_INVALID, "nq_fuse_glu: gate and up must share format, IN, OUT, group width and device");
@@ -1200,6 +1332,109 @@ int32_t nq_quantize_rows_i8(const void* x, int32_t x_dtype, int8_t* q, float* sc
     if (((uintptr_t)x & 15) || ((uintptr_t)q & 3))
         return fail(NQ_ERR_INVALID, "nq_quantize_rows_i8: x must be 16-byte and q 4-byte aligned");
     return launch_quantize_rows_i8(x, x_dtype, q, scales, M, K, (hipStream_t)stream);
+}
+
+int32_t nq_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* codes, float* scales, int32_t M, int32_t K,
+                                   void* stream) {
+    if (M < 0 || K <= 0) return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: M >= 0 and K > 0 are required");
+    if (x_dtype != NQ_DT_F32 && x_dtype != NQ_DT_BF16)
+        return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: x must be fp32 or bf16");
+    if (M == 0) return NQ_OK;
+    if (!x || !codes || !scales) return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: null pointer");
+    if (((uintptr_t)x & 15) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3))
+        return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: x and codes must be 16-byte and scales 4-byte aligned");
+    return launch_quantize_rows_fp8_block(x, x_dtype, codes, scales, M, K, (hipStream_t)stream);
+}
+
+int32_t nq_grad_input_fp8_block(nq_handle h, const uint8_t* gy, const float* gy_scale, void* gx, int32_t gx_dtype, int32_t M,
+                                void* stream) {
+    int32_t rc = check_handle(h, "nq_grad_input_fp8_block");
+    if (rc) return rc;
+    if ((rc = need_loaded(h, "vjp"))) return rc;
+    if (h->format != NQ_FMT_FP8_BLOCK) return fail(NQ_ERR_UNSUPPORTED, "nq_grad_input_fp8_block: FP8_BLOCK layers only");
+    if (!h->d_codes_t)
+        return fail(NQ_ERR_UNSUPPORTED, "nq_grad_input_fp8_block: the layer keeps no W^T (nq_create with NQ_FLAG_GRAD)");
+    if (M < 0) return fail(NQ_ERR_INVALID, "nq_grad_input_fp8_block: M must be >= 0");
+    if (M == 0) return NQ_OK;
+    if (!gy || !gy_scale || !gx) return fail(NQ_ERR_INVALID, "nq_grad_input_fp8_block: null gy, its scales or gx");
+    if (((uintptr_t)gy & 15) || ((uintptr_t)gy_scale & 3) || ((uintptr_t)gx & 3))
+        return fail(NQ_ERR_INVALID, "nq_grad_input_fp8_block: gy must be 16-byte, its scales and gx 4-byte aligned");
+    if (gx_dtype != NQ_DT_F32 && gx_dtype != NQ_DT_BF16)
+        return fail(NQ_ERR_INVALID, "nq_grad_input_fp8_block: gx must be fp32 or bf16");
+    nq_layer T;  // W^T as a layer (no ownership): the gradient is its product
+    T.format = NQ_FMT_FP8_BLOCK, T.in = h->out, T.out = h->in, T.group = FP8_BLOCK;
+    T.groups = (h->out - 1) / FP8_BLOCK + 1, T.row_bytes = (int64_t)T.groups * FP8_BLOCK;
+    T.loaded = true, T.device = h->device, T.d_codes = h->d_codes_t, T.d_scales = h->d_scales_t;
+    SegTable seg{};
+    seg.nseg = 1, seg.end[0] = T.out, seg.y[0] = gx;
+    const ForwardArgs a{&T, gy, NQ_DT_FP8_E4M3, gy_scale, gx, gx_dtype, M, nullptr, NQ_DT_F32, NQ_EPI_NONE, (hipStream_t)stream, seg};
+    return launch_fp8_block(a);
+}
+
+// what the two forms of the norm's forward ask of their common arguments
+static int32_t check_norm(const char* what, const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps,
+                          const float* mean, const float* rstd, int32_t M, int32_t D) {
+    const std::string w(what);
+    if (M < 0 || D <= 0) return fail(NQ_ERR_INVALID, w + ": M >= 0 and D > 0 are required");
+    if (x_dtype != NQ_DT_F32 && x_dtype != NQ_DT_BF16) return fail(NQ_ERR_INVALID, w + ": x must be fp32 or bf16");
+    if (!(eps >= 0.0f) || eps > 3.402823466e38f) return fail(NQ_ERR_INVALID, w + ": eps must be finite and not negative");
+    if ((mean == nullptr) != (rstd == nullptr)) return fail(NQ_ERR_INVALID, w + ": mean and rstd are given together or not at all");
+    if (M == 0) return NQ_OK;
+    if (!x) return fail(NQ_ERR_INVALID, w + ": null x");
+    if (((uintptr_t)x & 15) || ((uintptr_t)gamma & 15) || ((uintptr_t)beta & 15))
+        return fail(NQ_ERR_INVALID, w + ": x, gamma and beta must be 16-byte aligned");
+    return NQ_OK;
+}
+
+int32_t nq_layer_norm(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps, void* y,
+                      int32_t y_dtype, float* mean, float* rstd, int32_t M, int32_t D, void* stream) {
+    const int32_t rc = check_norm("nq_layer_norm", x, x_dtype, gamma, beta, eps, mean, rstd, M, D);
+    if (rc) return rc;
+    if (y_dtype != NQ_DT_F32 && y_dtype != NQ_DT_BF16) return fail(NQ_ERR_INVALID, "nq_layer_norm: y must be fp32 or bf16");
+    if (M == 0) return NQ_OK;
+    if (!y || ((uintptr_t)y & 15)) return fail(NQ_ERR_INVALID, "nq_layer_norm: y must be a 16-byte aligned device buffer");
+    if (y == x && y_dtype != x_dtype) return fail(NQ_ERR_INVALID, "nq_layer_norm: y may be x only where the types agree");
+    NormArgs a{x, x_dtype, gamma, beta, eps, y, y_dtype, nullptr, nullptr, mean, rstd, M, D};
+    return launch_layer_norm(a, (hipStream_t)stream);
+}
+
+int32_t nq_layer_norm_fp8_block(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps,
+                                uint8_t* codes, float* scales, float* mean, float* rstd, int32_t M, int32_t D, void* stream) {
+    const int32_t rc = check_norm("nq_layer_norm_fp8_block", x, x_dtype, gamma, beta, eps, mean, rstd, M, D);
+    if (rc) return rc;
+    if (M == 0) return NQ_OK;
+    if (!codes || !scales || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3))
+        return fail(NQ_ERR_INVALID, "nq_layer_norm_fp8_block: codes (16-byte aligned) and scales (4-byte) are needed");
+    NormArgs a{x, x_dtype, gamma, beta, eps, nullptr, NQ_DT_F32, codes, scales, mean, rstd, M, D};
+    return launch_layer_norm(a, (hipStream_t)stream);
+}
+
+int64_t nq_layer_norm_grad_workspace_bytes(int32_t M, int32_t D) {
+    return M <= 0 || D <= 0 ? 0 : layer_norm_grad_partial_bytes(M, D);
+}
+
+int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, const float* rstd, const float* gamma,
+                           const void* gy, int32_t gy_dtype, void* gx, int32_t gx_dtype, float* dgamma, float* dbeta,
+                           int32_t M, int32_t D, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (M < 0 || D <= 0) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: M >= 0 and D > 0 are required");
+    for (int32_t t : {x_dtype, gy_dtype, gx_dtype})
+        if (t != NQ_DT_F32 && t != NQ_DT_BF16) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: x, gy and gx must be fp32 or bf16");
+    if ((dgamma == nullptr) != (dbeta == nullptr))
+        return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: dgamma and dbeta are given together or not at all");
+    if (((uintptr_t)gamma & 15) || ((uintptr_t)dgamma & 15) || ((uintptr_t)dbeta & 15))
+        return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: gamma, dgamma and dbeta must be 16-byte aligned");
+    if (M > 0) {
+        if (!x || !mean || !rstd || !gy || !gx) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: null pointer");
+        if (((uintptr_t)x & 15) || ((uintptr_t)gy & 15) || ((uintptr_t)gx & 15))
+            return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: x, gy and gx must be 16-byte aligned");
+        if ((gx == gy && gx_dtype != gy_dtype) || (gx == x && gx_dtype != x_dtype))
+            return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: gx may be gy or x only where the types agree");
+        const int64_t need = dgamma ? layer_norm_grad_partial_bytes(M, D) : 0;
+        if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+            return fail(NQ_ERR_SIZE, "nq_layer_norm_grad: a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed");
+    }
+    const NormGradArgs a{x, gy, gx, x_dtype, gy_dtype, gx_dtype, mean, rstd, gamma, dgamma, dbeta, M, D, reinterpret_cast<float*>(workspace)};
+    return launch_layer_norm_grad(a, (hipStream_t)stream);
 }
 
 int32_t nq_cast_pad_bf16(const float* src, uint16_t* dst, int32_t rows, int32_t cols, int32_t cols_pad,

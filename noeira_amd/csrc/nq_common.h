@@ -15,6 +15,7 @@ namespace nq {
 
 constexpr int Q4_GROUP = 32;  // weights per Q4_0 group (noeira/nn/quant/q4_0.mojo:49)
 constexpr int Q4_BLOCK = 18;  // bytes per Q4_0 block   (noeira/nn/quant/q4_0.mojo:51)
+constexpr int FP8_BLOCK = 128;  // rows and columns of an FP8_BLOCK weight that share a scale
 constexpr int CHUNK = 16;     // bytes one lane loads per weight fetch (128-bit)
 
 // Sets the calling thread's error sentence and returns `code`.
@@ -48,6 +49,9 @@ hipError_t set_max_lds_once(LdsAttrOnce& st, const void* kernel, size_t bytes);
 //   W4_GROUP    codes  [OUT][IN/2]      (low nibble = even k)
 //               scales [OUT][G] fp16,   zps [OUT][G] uint8 (unpacked)
 //   FP8_E4M3    codes  [OUT][IN],       scale = one fp32
+//   FP8_BLOCK   codes  [ceil(OUT / 16)][G][2 KiB], G = ceil(IN / 128): one matrix-core operand of 16 rows x 128 k per
+//                      2 KiB (nq_fp8_block.hip), zeros behind OUT and IN; no row-ordered copy
+//               scales [ceil(OUT / 128)][G] fp32
 struct nq_layer {
     int32_t format = 0;
     int32_t in = 0;
@@ -80,6 +84,10 @@ struct nq_layer {
     // nq_fuse_glu: rows 2 n and 2 n + 1 are row n of the gate and of the up projection; the forward writes
     // [M, OUT / 2] = up * silu(gate) (epilogue NQ_EPI_SWIGLU) and nothing else
     bool glu = false;
+    // FP8_BLOCK layers made with NQ_FLAG_GRAD: W^T in the same layout (its rows are IN, its blocks run along OUT)
+    bool keep_grad = false;
+    uint8_t* d_codes_t = nullptr;
+    float* d_scales_t = nullptr;
 };
 
 namespace nq {
@@ -212,6 +220,46 @@ int32_t launch_tile8_i8(const ForwardArgs& a);
 double gemm8_estimate_us(int M, int N, int K, bool i8);  // what launch_gemm8 is expected to take, on the tile form it picks
 bool gemm8_applicable(const ForwardArgs& a);
 int32_t launch_gemm8(const ForwardArgs& a);
+
+// nq_fp8_block.hip: e4m3 weights with a scale per 128 x 128 block under e4m3 rows with a scale per 128 of K
+int32_t launch_fp8_block_repack(const uint8_t* codes, uint8_t* tiles, int32_t rows, int32_t cols, bool transpose, hipStream_t s);
+int32_t launch_fp8_block_scales_t(const float* scales, float* scales_t, int32_t nb, int32_t kb, hipStream_t s);
+int32_t launch_fp8_block_dequantize(const nq_layer* L, float* out, hipStream_t s);
+int32_t launch_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* codes, float* scales, int32_t M, int32_t K,
+                                       hipStream_t s);
+int32_t launch_fp8_block(const ForwardArgs& a);
+
+// nq_norm.hip: layer norm and its gradient
+struct NormArgs {
+    const void* x;
+    int32_t x_dtype;
+    const float* gamma;  // null: 1
+    const float* beta;   // null: 0
+    float eps;
+    void* y;             // null: codes / scales instead
+    int32_t y_dtype;
+    uint8_t* codes;
+    float* scales;
+    float* mean;         // both or neither
+    float* rstd;
+    int32_t M, D;
+};
+int32_t launch_layer_norm(const NormArgs& a, hipStream_t s);
+struct NormGradArgs {
+    const void* x;
+    const void* gy;
+    void* gx;
+    int32_t x_dtype, gy_dtype, gx_dtype;
+    const float* mean;
+    const float* rstd;
+    const float* gamma;  // null: 1
+    float* dgamma;       // both or neither
+    float* dbeta;
+    int32_t M, D;
+    float* partial;
+};
+int64_t layer_norm_grad_partial_bytes(int32_t M, int32_t D);
+int32_t launch_layer_norm_grad(const NormGradArgs& a, hipStream_t s);
 
 // nq_mlp.hip: three W8A8 layers in one launch
 int32_t launch_mlp3_w8a8(const nq_layer* l1, const nq_layer* l2, const nq_layer* l3, const float* x, float* y,

@@ -1,0 +1,361 @@
+// The block-scaled fp8 linear (NQ_FMT_FP8_BLOCK):
+//     y[m, n] = epi( sum_g sx[m, g] sw[n / 128, g] * sum_{k in block g} qx[m, k] qw[n, k]  + bias[n] )
+// with e4m3 codes qx, qw, one fp32 scale per activation row and 128 of K and one per 128 x 128 block of the weight.
+//
+// Why the block is the unit of everything here.  One v_mfma_f32_16x16x128_f8f6f4 multiplies 16 weight rows by 16
+// activation rows over exactly 128 k: its result is one block's sum for 256 outputs, summed by the matrix core from a
+// zero addend, and the two scales enter as ONE fused multiply-add per output and block.  With the weight as the
+// first operand a lane holds one activation row and four consecutive channels, so the row's scale is a lane's own
+// value, the weight's is the same for all lanes, and their product is made once per lane and block.
+//
+// Which matrix core.  The fp8 one does not sum in full fp32: it aligns a group's products to the largest and drops what
+// falls off the end.  On this GPU a block's sum is off by 1.3e-5 of the sums' root mean square for codes of N(0, 1)
+// values (all fp8 shapes alike; 5e-5 for uniformly drawn codes, at most 2.2e-4 of the sum of the products' magnitudes),
+// where the bf16 one is off by 1e-8.  Under a bf16 output's half step (2^-8) that is nothing; in an fp32 output it would
+// be the whole error.  So a call with an fp32 y decodes both operands' codes to bf16, which is exact, and multiplies on
+// v_mfma_f32_16x16x32_bf16 (half the rate, and 16 conversions per operand of 16 rows), and a call with a bf16 y
+// multiplies the codes.
+//
+// Weight layout.  The codes are kept only in the matrix core's operand order: tile (R, g) = rows 16 R .., k = 128 g ..
+// is 2 KiB at ((R * G) + g) * 2 KiB; lane l = r + 16 c of its first KiB holds row r's k = 32 c .. 32 c + 15, of its
+// second k = 32 c + 16 .. 32 c + 31, both 16 bytes at 16 l.  A wavefront's 128-bit load is one contiguous KiB and needs
+// no exchange between lanes.  Rows behind OUT and k behind IN are zero.
+#include "nq_common.h"
+#include "nq_fp8_quant.h"
+
+namespace nq {
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+
+// A lane's 32 bytes of an operand (16 rows x 128 k): as they are, or decoded to bf16 in four operands of 32 k each.
+// (A lane's k within an operand are the same 8 for both sides; which 8 they are does not matter to a sum.)
+template <bool EXACT>
+struct Operand;
+template <>
+struct Operand<false> {
+    i32x8 v;
+    __device__ __forceinline__ Operand(const i32x4& a, const i32x4& b) : v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]} {}
+};
+template <>
+struct Operand<true> {
+    bf16x8 v[4];
+    __device__ __forceinline__ Operand(const i32x4& a, const i32x4& b) {
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int w = s < 2 ? a[2 * s + h] : b[2 * (s - 2) + h];
+                const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+                const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
+                v[s][4 * h] = lo[0], v[s][4 * h + 1] = lo[1], v[s][4 * h + 2] = hi[0], v[s][4 * h + 3] = hi[1];
+            }
+    }
+};
+
+// one block's sums: 16 weight rows (result rows) x 16 activation rows (result columns)
+__device__ __forceinline__ f32x4 block_sum(const Operand<false>& w, const Operand<false>& x) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f32x4{}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 block_sum(const Operand<true>& w, const Operand<true>& x) {
+    f32x4 d = {};
+#pragma unroll
+    for (int s = 0; s < 4; s++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[s], x.v[s], d, 0, 0, 0);
+    return d;
+}
+
+// ---- load time ----------------------------------------------------------------------------------------------------
+
+// row-ordered codes [rows][cols] -> tiles; TRANSPOSE: of the transposed matrix (tile rows run along cols).  One thread
+// per 16 bytes of a tile.
+template <bool TRANSPOSE>
+__global__ __launch_bounds__(256) void fp8_block_repack_kernel(const uint8_t* __restrict__ codes, uint8_t* __restrict__ tiles,
+                                                               int32_t rows, int32_t cols, int64_t pieces) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= pieces) return;
+    const int32_t trows = TRANSPOSE ? cols : rows, tcols = TRANSPOSE ? rows : cols;
+    const int32_t G = (tcols - 1) / 128 + 1;
+    const int lane = (int)(t & 63), half = (int)(t >> 6) & 1;
+    const int64_t tile = t >> 7;
+    const int64_t row = tile / G * 16 + (lane & 15);
+    const int64_t k0 = tile % G * 128 + 32 * (lane >> 4) + 16 * half;
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (row < trows) {
+#pragma unroll
+        for (int b = 0; b < 16; b++) {
+            const int64_t k = k0 + b;
+            if (k < tcols) w[b / 4] |= (uint32_t)codes[TRANSPOSE ? k * cols + row : row * cols + k] << (8 * (b % 4));
+        }
+    }
+    reinterpret_cast<uint4*>(tiles)[t] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__global__ __launch_bounds__(256) void fp8_block_scales_t_kernel(const float* __restrict__ s, float* __restrict__ st, int32_t nb,
+                                                                 int32_t kb) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t < (int64_t)nb * kb) st[t % kb * nb + t / kb] = s[t];
+}
+
+// one thread per 16 values of a row
+__global__ __launch_bounds__(256) void fp8_block_dequantize_kernel(const uint8_t* __restrict__ tiles, const float* __restrict__ ws,
+                                                                   float* __restrict__ out, int32_t N, int32_t K, int32_t G) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int32_t pieces = K / 16;
+    if (t >= (int64_t)N * pieces) return;
+    const int64_t n = t / pieces;
+    const int32_t k = (int32_t)(t % pieces) * 16, g = k / 128, c = k / 32 % 4, half = k / 16 % 2;
+    const uint4 v = *reinterpret_cast<const uint4*>(tiles + (n / 16 * G + g) * 2048 + half * 1024 + (n % 16 + 16 * c) * 16);
+    const float s = ws[n / 128 * G + g];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float4* o = reinterpret_cast<float4*>(out + n * K + k);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        o[i] = make_float4(__builtin_amdgcn_cvt_f32_fp8((int)w[i], 0) * s, __builtin_amdgcn_cvt_f32_fp8((int)w[i], 1) * s,
+                           __builtin_amdgcn_cvt_f32_fp8((int)w[i], 2) * s, __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3) * s);
+}
+
+// ---- activations --------------------------------------------------------------------------------------------------
+
+// 16 lanes per block of 128.  VEC (K % 8 == 0): a lane's 8 values are adjacent, 128-bit loads and one 64-bit store;
+// otherwise every 16th value, element by element.
+template <bool BF16, bool VEC>
+__global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void* __restrict__ x, uint8_t* __restrict__ codes,
+                                                                      float* __restrict__ scales, int32_t K, uint32_t G,
+                                                                      uint32_t blocks) {
+    const uint32_t b = blockIdx.x * 16u + (threadIdx.x >> 4);
+    if (b >= blocks) return;  // (16 lanes leave together: a DPP row)
+    const uint32_t m = b / G, g = b - m * G;
+    const int l = threadIdx.x & 15;
+    const int64_t base = (int64_t)m * K;
+    float v[8];
+    float s;
+    if constexpr (VEC) {
+        const int32_t k = (int32_t)g * 128 + 8 * l;
+        const bool in = k < K;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = 0.0f;
+        if (in) {
+            if constexpr (BF16) {
+                const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + base + k);
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+            } else {
+                const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + base + k);
+                const float4 a = p[0], c = p[1];
+                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = c.x, v[5] = c.y, v[6] = c.z, v[7] = c.w;
+            }
+        }
+        const uint2 q = quantize_block16(v, s);
+        if (in) *reinterpret_cast<uint2*>(codes + base + k) = q;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int32_t k = (int32_t)g * 128 + 16 * i + l;
+            v[i] = k >= K ? 0.0f
+                          : BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(x)[base + k] << 16)
+                                 : reinterpret_cast<const float*>(x)[base + k];
+        }
+        const uint2 q = quantize_block16(v, s);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int32_t k = (int32_t)g * 128 + 16 * i + l;
+            if (k < K) codes[base + k] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+        }
+    }
+    if (l == 0) scales[b] = s;
+}
+
+// ---- the product --------------------------------------------------------------------------------------------------
+
+struct BlockParams {
+    const uint8_t* x;
+    const uint8_t* w;
+    const float* xs;
+    const float* ws;
+    const void* bias;
+    int32_t M, N, K, G;
+    int32_t tiles_m;
+    int32_t y_dtype, bias_dtype, relu;
+    SegTable seg;
+};
+
+__device__ __forceinline__ uint16_t bf16_bits(float v) {
+    uint32_t bits = __float_as_uint(v);
+    if ((bits & 0x7FFFFFFFu) > 0x7F800000u) return 0x7FC0;
+    return (uint16_t)((bits + 0x7FFFu + ((bits >> 16) & 1u)) >> 16);
+}
+
+// MT x NT MFMA tiles of 16 x 16 per workgroup, the blocks of K dealt over KW wavefronts, whose sums meet in LDS in
+// wavefront order (bit-repeatable).  U: blocks requested together.
+template <int MT, int NT, int KW, int U, bool EXACT>
+__global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockParams p) {
+    constexpr int ROWS = 16 * MT, CH = 16 * NT;
+    __shared__ __attribute__((aligned(16))) float part[KW][ROWS][CH + 4];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, c = lane >> 4;
+    const int tn = blockIdx.x / p.tiles_m, tm = blockIdx.x - tn * p.tiles_m;
+    const int m0 = tm * ROWS, n0 = tn * CH;
+    const int row_tiles = (p.N + 15) / 16;
+
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // rows behind M repeat the last one: their results are columns of their own, never stored
+    int64_t mrow[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) mrow[i] = min(m0 + 16 * i + r, p.M - 1);
+    const uint8_t* wtile[NT];
+    const float* wscale[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        const int R = min(n0 / 16 + j, row_tiles - 1);
+        wtile[j] = p.w + (int64_t)R * p.G * 2048 + lane * 16;
+        wscale[j] = p.ws + (int64_t)(R / 8) * p.G;
+    }
+    for (int g0 = wave; g0 < p.G; g0 += KW * U) {
+        i32x4 xv[U][MT][2], wv[U][NT][2];
+        float sx[U][MT], sw[U][NT];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int g = min(g0 + u * KW, p.G - 1);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) wv[u][j][e] = *reinterpret_cast<const i32x4*>(wtile[j] + (int64_t)g * 2048 + e * 1024);
+                sw[u][j] = wscale[j][g];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    // (K is a multiple of 16: a piece lies in the row or behind it, and what lies behind counts as zero)
+                    const int k = 128 * g + 32 * c + 16 * e;
+                    const i32x4 v = *reinterpret_cast<const i32x4*>(p.x + mrow[i] * p.K + (k < p.K ? k : 0));
+                    xv[u][i][e] = k < p.K ? v : i32x4{0, 0, 0, 0};
+                }
+                sx[u][i] = p.xs[mrow[i] * p.G + g];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (g0 + u * KW < p.G) {
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const Operand<EXACT> w(wv[u][j][0], wv[u][j][1]);
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        const Operand<EXACT> x(xv[u][i][0], xv[u][i][1]);
+                        const f32x4 d = block_sum(w, x);
+                        const float s = sx[u][i] * sw[u][j];
+#pragma unroll
+                        for (int t = 0; t < 4; t++) acc[i][j][t] = fmaf(d[t], s, acc[i][j][t]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) *reinterpret_cast<f32x4*>(&part[wave][16 * i + r][16 * j + 4 * c]) = acc[i][j];
+    __syncthreads();
+    for (int o = threadIdx.x; o < ROWS * CH; o += 64 * KW) {
+        const int row = o / CH, ch = o % CH;
+        const int m = m0 + row, n = n0 + ch;
+        if (m >= p.M || n >= p.N) continue;
+        float z = part[0][row][ch];
+#pragma unroll
+        for (int w = 1; w < KW; w++) z += part[w][row][ch];
+        if (p.bias)
+            z += p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[n]
+                                           : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[n] << 16);
+        if (p.relu) z = z > 0.0f ? z : 0.0f;
+        void* y;
+        int width, col;
+        seg_lookup(p.seg, n, y, width, col);
+        if (p.y_dtype == NQ_DT_F32)
+            reinterpret_cast<float*>(y)[(int64_t)m * width + col] = z;
+        else
+            reinterpret_cast<uint16_t*>(y)[(int64_t)m * width + col] = bf16_bits(z);
+    }
+}
+
+template <int MT, int NT, int KW, int U>
+int32_t launch_tile(BlockParams p, hipStream_t s) {
+    p.tiles_m = (p.M + 16 * MT - 1) / (16 * MT);
+    const int64_t grid = (int64_t)p.tiles_m * ((p.N + 16 * NT - 1) / (16 * NT));
+    if (grid > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
+    if (p.y_dtype == NQ_DT_F32)
+        hipLaunchKernelGGL((fp8_block_tile_kernel<MT, NT, KW, U, true>), dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
+    else
+        hipLaunchKernelGGL((fp8_block_tile_kernel<MT, NT, KW, U, false>), dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
+    NQ_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+}  // namespace
+
+int32_t launch_fp8_block_repack(const uint8_t* codes, uint8_t* tiles, int32_t rows, int32_t cols, bool transpose, hipStream_t s) {
+    const int64_t trows = transpose ? cols : rows, tcols = transpose ? rows : cols;
+    const int64_t pieces = (trows + 15) / 16 * ((tcols + 127) / 128) * 128;
+    if (transpose)
+        hipLaunchKernelGGL((fp8_block_repack_kernel<true>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, codes, tiles, rows, cols, pieces);
+    else
+        hipLaunchKernelGGL((fp8_block_repack_kernel<false>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, codes, tiles, rows, cols, pieces);
+    NQ_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+int32_t launch_fp8_block_scales_t(const float* scales, float* scales_t, int32_t nb, int32_t kb, hipStream_t s) {
+    const int64_t n = (int64_t)nb * kb;
+    hipLaunchKernelGGL(fp8_block_scales_t_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, scales, scales_t, nb, kb);
+    NQ_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+int32_t launch_fp8_block_dequantize(const nq_layer* L, float* out, hipStream_t s) {
+    const int64_t n = (int64_t)L->out * (L->in / 16);
+    hipLaunchKernelGGL(fp8_block_dequantize_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, L->d_codes,
+                       reinterpret_cast<const float*>(L->d_scales), out, L->out, L->in, L->groups);
+    NQ_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+int32_t launch_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* codes, float* scales, int32_t M, int32_t K,
+                                       hipStream_t s) {
+    const int64_t G = (K - 1) / 128 + 1, blocks = M * G;
+    if (blocks > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: more than 2^31 - 1 blocks of 128");
+    const bool bf16 = x_dtype == NQ_DT_BF16, vec = K % 8 == 0;
+#define NQ_QB(B, V)                                                                                                        \
+    hipLaunchKernelGGL((quantize_rows_fp8_block_kernel<B, V>), dim3((unsigned)((blocks + 15) / 16)), dim3(256), 0, s, x,   \
+                       codes, scales, K, (uint32_t)G, (uint32_t)blocks)
+    if (bf16 && vec) NQ_QB(true, true);
+    else if (bf16) NQ_QB(true, false);
+    else if (vec) NQ_QB(false, true);
+    else NQ_QB(false, false);
+#undef NQ_QB
+    NQ_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+int32_t launch_fp8_block(const ForwardArgs& a) {
+    const nq_layer* L = a.L;
+    BlockParams p{};
+    p.x = reinterpret_cast<const uint8_t*>(a.x), p.w = L->d_codes;
+    p.xs = a.x_scale, p.ws = reinterpret_cast<const float*>(L->d_scales), p.bias = a.bias;
+    p.M = a.M, p.N = L->out, p.K = L->in, p.G = L->groups;
+    p.y_dtype = a.y_dtype, p.bias_dtype = a.bias_dtype, p.relu = a.epilogue == NQ_EPI_RELU;
+    p.seg = a.seg;
+    return launch_tile<1, 1, 4, 4>(p, a.stream);
+}
+
+}  // namespace nq

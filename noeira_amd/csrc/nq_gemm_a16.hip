@@ -1099,7 +1099,7 @@ float gemm_a16_best_estimate_us(int32_t format, bool xf32, int M, int N, int K) 
 
 bool gemm_a16_applicable(const ForwardArgs& a) {
     const nq_layer* L = a.L;
-    if (a.x_dtype != NQ_DT_F32 && a.x_dtype != NQ_DT_BF16) return false;
+    if ((a.x_dtype != NQ_DT_F32 && a.x_dtype != NQ_DT_BF16) || L->format == NQ_FMT_FP8_BLOCK) return false;
     const bool bytes = L->format == NQ_FMT_W8_CHANNEL || L->format == NQ_FMT_FP8_E4M3;
     if (L->in % (bytes ? 16 : 32) != 0) return false;
     // the kernel addresses each operand with 32-bit byte offsets

@@ -222,6 +222,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t* __restri
 }
 
 int32_t launch_dequantize(const nq_layer* L, float* out, hipStream_t s) {
+    if (L->format == NQ_FMT_FP8_BLOCK) return launch_fp8_block_dequantize(L, out, s);
     const int epc = (L->format == NQ_FMT_Q4_0 || L->format == NQ_FMT_W4_GROUP) ? 32 : 16;
     int64_t n = (int64_t)L->out * (L->in / epc);
     if (n == 0) return NQ_OK;

@@ -10,6 +10,7 @@ The helpers here build the byte layouts of the extension formats that
             zps    [N, ceil(G/2)]  byte i = group 2i (low nibble) | group 2i+1 (high)
             value  = (q - z) * fp32(s)
   FP8_E4M3  OCP e4m3fn codes (max finite 448, no infinities), one fp32 scale
+  FP8_BLOCK e4m3fn codes [N, K], one fp32 scale per block of 128 x 128: [ceil(N/128), ceil(K/128)]
 """
 from __future__ import annotations
 
@@ -67,3 +68,19 @@ def encode_e4m3(x: np.ndarray) -> np.ndarray:
 
     t = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).clamp_(-448.0, 448.0)
     return t.to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+
+
+def quantize_fp8_block(w: np.ndarray):
+    """An fp32 [N, K] weight in blocks of 128 x 128 (the last ones as large as is left): s = absmax / 448 (1 where a
+    block is zero, never below 2^-126), codes e4m3(w / s); returns (codes uint8 [N, K], scales [NB, KB])."""
+    w = np.ascontiguousarray(w, dtype=np.float32)
+    N, K = w.shape
+    nb, kb = -(-N // 128), -(-K // 128)
+    pad = np.zeros((nb * 128, kb * 128), np.float32)
+    pad[:N, :K] = w
+    t = pad.reshape(nb, 128, kb, 128)
+    top = np.abs(t).max(axis=(1, 3))
+    s = np.maximum(top / np.float32(448), np.float32(2.0 ** -126)).astype(np.float32)
+    s[top == 0] = 1.0
+    q = (t / s[:, None, :, None]).reshape(nb * 128, kb * 128)[:N, :K]
+    return encode_e4m3(q), s

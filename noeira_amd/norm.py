@@ -1,0 +1,120 @@
+"""Layer norm in front of a quantized linear, over the C ABI.
+
+``LayerNorm`` normalises rows of DIM values and hands them on in the form the next layer takes: fp32 or bf16
+(``forward``), or the e4m3 codes and block scales of an ``FP8BlockLinear`` (``forward_fp8``: norm and quantisation in one
+launch, the normalised values are never stored).  ``vjp`` is the gradient of its input, gamma and beta.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import numpy as np
+import torch
+
+from . import _lib as L
+from .qlinear import _TORCH_DT, _check_dev, _dev_ptr, _need_gpu, _stream_ptr
+
+
+class LayerNorm:
+    """y[M, DIM] = (x - mean) / sqrt(var + eps) * gamma + beta; gamma, beta fp32 [DIM] on the device, ones and zeros
+    until ``set_params``."""
+
+    def __init__(self, DIM: int, eps: float = 1e-5):
+        if DIM < 1:
+            raise L.NQError(L.NQ_ERR_INVALID, "LayerNorm: DIM must be positive")
+        self.DIM, self.eps = int(DIM), float(eps)
+        self.gamma = torch.ones((DIM,), dtype=torch.float32, device="cuda")
+        self.beta = torch.zeros((DIM,), dtype=torch.float32, device="cuda")
+
+    @classmethod
+    def make(cls, DIM: int, eps: float = 1e-5, target: str = "gpu") -> "LayerNorm":
+        _need_gpu(target)
+        return cls(DIM, eps)
+
+    def set_params(self, gamma, beta):
+        """fp32 [DIM] each: arrays or tensors; copied."""
+        new = []
+        for name, v in (("gamma", gamma), ("beta", beta)):
+            t = v if isinstance(v, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(v, dtype=np.float32))
+            if tuple(t.shape) != (self.DIM,):
+                raise L.NQError(L.NQ_ERR_SIZE, f"LayerNorm.set_params: {name} is {list(t.shape)}, expected [{self.DIM}]")
+            new.append(t)
+        self.gamma.copy_(new[0])
+        self.beta.copy_(new[1])
+
+    def _rows(self, x: torch.Tensor, what: str) -> int:
+        _check_dev(x, f"LayerNorm.{what}: x", tuple(_TORCH_DT))
+        _check_dev(self.gamma, f"LayerNorm.{what}: gamma")
+        if x.numel() % self.DIM:
+            raise L.NQError(L.NQ_ERR_INVALID, f"LayerNorm.{what}: x has {x.numel()} values, not a multiple of DIM = {self.DIM}")
+        return x.numel() // self.DIM
+
+    def _forward(self, x, out, out_dtype, stats, what):
+        M = self._rows(x, what)
+        if out is not None:
+            out_dtype = out.dtype if out_dtype is None else out_dtype
+            _check_dev(out, f"LayerNorm.{what}: out", out_dtype, M * self.DIM)
+        out_dtype = x.dtype if out_dtype is None else out_dtype
+        if out_dtype not in _TORCH_DT:
+            raise L.NQError(L.NQ_ERR_INVALID, f"LayerNorm.{what}: y must be fp32 or bf16")
+        if out is None:
+            out = torch.empty((M, self.DIM), dtype=out_dtype, device=x.device)
+        mean = torch.empty((M,), dtype=torch.float32, device=x.device) if stats else None
+        rstd = torch.empty_like(mean) if stats else None
+        L.check(L.lib().nq_layer_norm(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(self.gamma), _dev_ptr(self.beta),
+                                      C.c_float(self.eps), _dev_ptr(out), _TORCH_DT[out_dtype], _dev_ptr(mean), _dev_ptr(rstd),
+                                      M, self.DIM, _stream_ptr()))
+        return out, mean, rstd
+
+    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """y [M, DIM], of x's type unless `out_dtype` (fp32 or bf16) says otherwise; `out` may be x itself."""
+        return self._forward(x, out, out_dtype, False, "forward")[0]
+
+    def forward_train(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None):
+        """(y, mean, rstd): `forward` with the statistics fp32 [M] that ``vjp`` takes."""
+        return self._forward(x, out, out_dtype, True, "forward_train")
+
+    def _forward_fp8(self, x, stats, what):
+        M = self._rows(x, what)
+        codes = torch.empty((M, self.DIM), dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty((M, -(-self.DIM // 128)), dtype=torch.float32, device=x.device)
+        mean = torch.empty((M,), dtype=torch.float32, device=x.device) if stats else None
+        rstd = torch.empty_like(mean) if stats else None
+        L.check(L.lib().nq_layer_norm_fp8_block(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(self.gamma), _dev_ptr(self.beta),
+                                                C.c_float(self.eps), _dev_ptr(codes), _dev_ptr(scales), _dev_ptr(mean),
+                                                _dev_ptr(rstd), M, self.DIM, _stream_ptr()))
+        return codes, scales, mean, rstd
+
+    def forward_fp8(self, x: torch.Tensor):
+        """(codes [M, DIM], scales [M, ceil(DIM/128)]): what ``quantize_rows_fp8_block`` makes of the fp32 result."""
+        return self._forward_fp8(x, False, "forward_fp8")[:2]
+
+    def forward_fp8_train(self, x: torch.Tensor):
+        """(codes, scales, mean, rstd)."""
+        return self._forward_fp8(x, True, "forward_fp8_train")
+
+    def vjp(self, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, grad_output: torch.Tensor,
+            grad_input: Optional[torch.Tensor] = None, params: bool = True):
+        """(grad_input [M, DIM] of x's type, dgamma, dbeta fp32 [DIM]) from the forward's input and statistics;
+        ``params=False`` (a frozen norm): no sums over the rows, dgamma and dbeta are None."""
+        M = self._rows(x, "vjp")
+        _check_dev(grad_output, "LayerNorm.vjp: grad_output", tuple(_TORCH_DT), M * self.DIM)
+        _check_dev(mean, "LayerNorm.vjp: mean", torch.float32, M)
+        _check_dev(rstd, "LayerNorm.vjp: rstd", torch.float32, M)
+        if grad_input is None:
+            grad_input = torch.empty((M, self.DIM), dtype=x.dtype, device=x.device)
+        else:
+            _check_dev(grad_input, "LayerNorm.vjp: grad_input", tuple(_TORCH_DT), M * self.DIM)
+        dg = db = ws = None
+        n = 0
+        if params:
+            dg = torch.empty((self.DIM,), dtype=torch.float32, device=x.device)
+            db = torch.empty_like(dg)
+            n = int(L.lib().nq_layer_norm_grad_workspace_bytes(M, self.DIM))
+            ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
+        L.check(L.lib().nq_layer_norm_grad(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(mean), _dev_ptr(rstd), _dev_ptr(self.gamma),
+                                           _dev_ptr(grad_output), _TORCH_DT[grad_output.dtype], _dev_ptr(grad_input),
+                                           _TORCH_DT[grad_input.dtype], _dev_ptr(dg), _dev_ptr(db), M, self.DIM, _dev_ptr(ws),
+                                           n, _stream_ptr()))
+        return grad_input, dg, db

@@ -46,6 +46,17 @@ def _dev_ptr(t: Optional[torch.Tensor]) -> C.c_void_p:
     return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
 
 
+def _check_dev(t: torch.Tensor, what: str, dtype=None, numel=None):
+    """A contiguous tensor on the current device (the stream the call goes to is that device's), of this type and size."""
+    if not t.is_cuda or t.device.index != torch.cuda.current_device() or not t.is_contiguous():
+        raise L.NQError(L.NQ_ERR_INVALID, what + " must be a contiguous tensor on the current device")
+    if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        raise L.NQError(L.NQ_ERR_INVALID, what + " must be " + " or ".join(str(d) for d in (dtype if isinstance(dtype, tuple) else (dtype,))))
+    if numel is not None and t.numel() != numel:
+        raise L.NQError(L.NQ_ERR_SIZE, f"{what} has {t.numel()} values, expected {numel}")
+    return t
+
+
 def _check_x(x: torch.Tensor, IN: int, what: str):
     if not x.is_cuda or not x.is_contiguous():
         raise L.NQError(L.NQ_ERR_INVALID, what + ": x must be a contiguous device tensor")
@@ -59,12 +70,12 @@ class _Layer:
 
     FORMAT = -1
 
-    def __init__(self, IN: int, OUT: int, group: int = 0, tile_copy: bool = True, prefer_tile: bool = False):
+    def __init__(self, IN: int, OUT: int, group: int = 0, tile_copy: bool = True, prefer_tile: bool = False, flags: int = 0):
         """tile_copy=False (NQ_FLAG_NO_TILE_COPY): a large layer does not keep the second,
         matrix-core-ordered copy of its codes that its single-row calls stream faster."""
         self.IN, self.OUT, self.group = int(IN), int(OUT), int(group)
         h = C.c_void_p()
-        flags = (0 if tile_copy else L.FLAG_NO_TILE_COPY) | (L.FLAG_PREFER_TILE if prefer_tile else 0)
+        flags |= (0 if tile_copy else L.FLAG_NO_TILE_COPY) | (L.FLAG_PREFER_TILE if prefer_tile else 0)
         L.check(L.lib().nq_create(C.byref(h), self.FORMAT, self.IN, self.OUT, self.group, flags))
         self._h = h
         self._loaded = False
@@ -379,6 +390,102 @@ class FP8Linear(_Layer):
         return self._forward(x, _TORCH_DT[x.dtype], None, out, out_dtype, bias, epilogue, "FP8Linear.forward_a16")
 
 
+class FP8BlockLinear(_Layer):
+    """OCP e4m3fn weight [OUT, IN] with one fp32 scale per block of 128 x 128; activations e4m3fn with one fp32 scale per
+    row and 128 of IN (`quantize_rows_fp8_block`, or a `LayerNorm`'s `forward_fp8`); fp32 accumulation of the blocks'
+    sums under their scales; bf16 or fp32 output.  ``grad=True`` keeps W^T beside W, which `vjp` reads."""
+
+    FORMAT = L.FMT_FP8_BLOCK
+
+    def __init__(self, IN: int, OUT: int, grad: bool = False):
+        super().__init__(IN, OUT, 128, flags=L.FLAG_GRAD if grad else 0)
+        self.grad = grad
+        self.KB, self.NB = -(-IN // 128), -(-OUT // 128)
+
+    @classmethod
+    def from_linear(cls, w_in_out, bias=None, grad: bool = False) -> "FP8BlockLinear":
+        """`Linear[IN, OUT]`'s W [IN, OUT] transposed and encoded as e4m3fn in blocks of 128 x 128 (absmax / 448); the
+        fp32 bias, if any, is kept on the device and added by forward."""
+        from . import formats as F
+
+        IN, OUT = np.asarray(w_in_out).shape
+        lin = cls(IN, OUT, grad=grad)
+        wt, lin.bias = cls._linear_params(w_in_out, bias, IN, OUT, "FP8BlockLinear.from_linear")
+        lin.set_weight(*F.quantize_fp8_block(wt))
+        return lin
+
+    def set_weight(self, w_codes, scales):
+        """codes [OUT, IN] and fp32 scales [ceil(OUT/128), ceil(IN/128)]: numpy arrays, or tensors on the current
+        device (no logical bytes are kept for ``blocks`` then)."""
+        what = f"FP8BlockLinear.set_weight: expected [{self.OUT}, {self.IN}] codes and [{self.NB}, {self.KB}] scales"
+        if isinstance(w_codes, torch.Tensor) or isinstance(scales, torch.Tensor):
+            if not isinstance(w_codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+                raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.set_weight: codes and scales are both arrays or both tensors")
+            if tuple(w_codes.shape) != (self.OUT, self.IN) or tuple(scales.shape) != (self.NB, self.KB):
+                raise L.NQError(L.NQ_ERR_SIZE, what)
+            _check_dev(w_codes, "FP8BlockLinear.set_weight: codes", (torch.uint8, torch.float8_e4m3fn))
+            _check_dev(scales, "FP8BlockLinear.set_weight: scales", torch.float32)
+            L.check(L.lib().nq_set_weight_fp8_block_dev(self._h, _dev_ptr(w_codes), _dev_ptr(scales), _stream_ptr()))
+        else:
+            w = np.ascontiguousarray(w_codes, dtype=np.uint8)
+            s = np.ascontiguousarray(scales, dtype=np.float32)
+            if w.size != self.IN * self.OUT or s.size != self.NB * self.KB:
+                raise L.NQError(L.NQ_ERR_SIZE, what)
+            L.check(L.lib().nq_set_weight_fp8_block(self._h, w.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p),
+                                                    _stream_ptr()))
+        self._loaded = True
+
+    @staticmethod
+    def _codes(codes: torch.Tensor, scales: torch.Tensor, K: int, what: str) -> int:
+        """Checks quantised rows [M, K] and their scales [M, ceil(K/128)]; returns M."""
+        _check_dev(codes, what + ": the codes", (torch.uint8, torch.float8_e4m3fn))
+        M = _check_x(codes, K, what)
+        _check_dev(scales, what + ": the scales", torch.float32, M * (-(-K // 128)))
+        return M
+
+    def forward_a8(self, x_codes, x_scales, bias=None, epilogue="none", out=None, out_dtype=torch.bfloat16):
+        """x_codes: e4m3fn (or uint8) [M, IN]; x_scales: fp32 [M, ceil(IN/128)]."""
+        M = self._codes(x_codes, x_scales, self.IN, "FP8BlockLinear.forward_a8")
+        if out_dtype not in _TORCH_DT:
+            raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.forward_a8: y must be fp32 or bf16")
+        if bias is not None:
+            _check_dev(bias, "FP8BlockLinear.forward_a8: bias")
+        if out is not None:
+            _check_dev(out, "FP8BlockLinear.forward_a8: out", out_dtype, M * self.OUT)
+        return self._forward(x_codes, L.DT_FP8_E4M3, x_scales, out, out_dtype, bias, epilogue, "FP8BlockLinear.forward_a8")
+
+    def forward(self, x: torch.Tensor, bias=None, epilogue="none", out=None, out_dtype=torch.bfloat16):
+        """fp32 or bf16 activations: quantised per row and block of 128, then the product (two launches)."""
+        if x.dtype not in _TORCH_DT:
+            raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.forward: x must be fp32 or bf16")
+        M = _check_x(x, self.IN, "FP8BlockLinear.forward")
+        return self.forward_a8(*quantize_rows_fp8_block(x.view(M, self.IN)), bias=bias, epilogue=epilogue, out=out,
+                               out_dtype=out_dtype)
+
+    def vjp_a8(self, gy_codes, gy_scales, grad_input: Optional[torch.Tensor] = None, out_dtype=torch.float32) -> torch.Tensor:
+        """grad_input = grad_output @ deq(W), overwriting it; grad_output as e4m3fn codes [M, OUT] with scales
+        [M, ceil(OUT/128)].  The layer must have been made with ``grad=True``."""
+        M = self._codes(gy_codes, gy_scales, self.OUT, "FP8BlockLinear.vjp_a8")
+        if out_dtype not in _TORCH_DT:
+            raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.vjp_a8: gx must be fp32 or bf16")
+        if grad_input is None:
+            grad_input = torch.empty((M, self.IN), dtype=out_dtype, device=gy_codes.device)
+        else:
+            _check_dev(grad_input, "FP8BlockLinear.vjp_a8: grad_input", out_dtype, M * self.IN)
+        L.check(L.lib().nq_grad_input_fp8_block(self._h, _dev_ptr(gy_codes), _dev_ptr(gy_scales), _dev_ptr(grad_input),
+                                                _TORCH_DT[out_dtype], M, _stream_ptr()))
+        return grad_input
+
+    def vjp(self, forward_input: Optional[torch.Tensor], grad_output: torch.Tensor,
+            grad_input: Optional[torch.Tensor] = None, out_dtype=torch.float32) -> torch.Tensor:
+        """`vjp_a8` of an fp32 or bf16 grad_output, quantised per row and block of 128 of OUT first (the gradient is
+        linear in it and does not depend on forward_input, which may be None)."""
+        if grad_output.dtype not in _TORCH_DT:
+            raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.vjp: grad_output must be fp32 or bf16")
+        M = _check_x(grad_output, self.OUT, "FP8BlockLinear.vjp")
+        return self.vjp_a8(*quantize_rows_fp8_block(grad_output.view(M, self.OUT)), grad_input=grad_input, out_dtype=out_dtype)
+
+
 class FusedRows:
     """Up to four loaded layers that read the same activations (q|k|v, gate|up
     of a decoder layer: `DecoderLayerWeights.proj_fwd`, layer_weights.mojo:455-508)
@@ -416,7 +523,7 @@ class FusedRows:
     def forward(self, x: torch.Tensor, x_scale: Optional[torch.Tensor] = None, outs=None, bias=None,
                 epilogue: str = "none", out_dtype: torch.dtype = torch.float32):
         """Returns the list of per-part outputs.  x: fp32/bf16 [M, IN], or e4m3fn
-        codes with `x_scale` for fused FP8Linear layers."""
+        codes with `x_scale` for fused FP8Linear and FP8BlockLinear layers."""
         if x.dtype == torch.float8_e4m3fn:
             x = x.view(torch.uint8)
         if x.dtype == torch.uint8:
@@ -426,6 +533,8 @@ class FusedRows:
         else:
             raise L.NQError(L.NQ_ERR_INVALID, "FusedRows.forward: x must be fp32, bf16 or e4m3fn codes")
         M = _check_x(x, self.IN, "FusedRows.forward")
+        if self._kind is FP8BlockLinear:
+            FP8BlockLinear._codes(x, x_scale, self.IN, "FusedRows.forward")
         if outs is None:
             outs = [torch.empty((M, n), dtype=out_dtype, device=x.device) for n in self.OUTS]
         y_dt = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}[out_dtype]
@@ -565,6 +674,26 @@ def quantize_rows_i8(x: torch.Tensor, q: Optional[torch.Tensor] = None, scales: 
     L.check(L.lib().nq_quantize_rows_i8(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(q), _dev_ptr(scales), M, K,
                                         _stream_ptr()))
     return q, scales
+
+
+def quantize_rows_fp8_block(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
+    """Per row and block of 128 of K: (e4m3fn codes [M, K], scales fp32 [M, ceil(K/128)]) of an fp32 / bf16 [M, K]."""
+    if x.dtype not in _TORCH_DT or x.dim() != 2 or not x.is_contiguous():
+        raise L.NQError(L.NQ_ERR_INVALID, "quantize_rows_fp8_block: x must be a contiguous fp32/bf16 [M, K] device tensor")
+    _check_dev(x, "quantize_rows_fp8_block: x")
+    M, K = x.shape
+    G = -(-K // 128)
+    if codes is None:
+        codes = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
+    else:
+        _check_dev(codes, "quantize_rows_fp8_block: codes", (torch.uint8, torch.float8_e4m3fn), M * K)
+    if scales is None:
+        scales = torch.empty((M, G), dtype=torch.float32, device=x.device)
+    else:
+        _check_dev(scales, "quantize_rows_fp8_block: scales", torch.float32, M * G)
+    L.check(L.lib().nq_quantize_rows_fp8_block(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(codes), _dev_ptr(scales), M, K,
+                                               _stream_ptr()))
+    return codes, scales
 
 
 def cast_pad_bf16(x: torch.Tensor, cols_pad: int) -> torch.Tensor:
