@@ -1421,8 +1421,8 @@ int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, co
         if (t != NQ_DT_F32 && t != NQ_DT_BF16) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: x, gy and gx must be fp32 or bf16");
     if ((dgamma == nullptr) != (dbeta == nullptr))
         return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: dgamma and dbeta are given together or not at all");
-    if (((uintptr_t)gamma & 15) || ((uintptr_t)dgamma & 15) || ((uintptr_t)dbeta & 15))
-        return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: gamma, dgamma and dbeta must be 16-byte aligned");
+    if (((uintptr_t)gamma & 15) || ((uintptr_t)dgamma & 3) || ((uintptr_t)dbeta & 3))
+        return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: gamma must be 16-byte, dgamma and dbeta 4-byte aligned");
     if (M > 0) {
         if (!x || !mean || !rstd || !gy || !gx) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: null pointer");
         if (((uintptr_t)x & 15) || ((uintptr_t)gy & 15) || ((uintptr_t)gx & 15))

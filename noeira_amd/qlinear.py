@@ -30,8 +30,14 @@ Q4_BLOCK = 18
 _TORCH_DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}
 
 
-def _stream_ptr() -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+# (the stream's address without a Stream object around it: 0.3 us a call instead of 2.8)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_ptr() -> int:
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _need_gpu(target: str):
@@ -42,15 +48,15 @@ def _need_gpu(target: str):
         raise L.NQError(L.NQ_ERR_HIP, "noeira_amd: no HIP device is visible")
 
 
-def _dev_ptr(t: Optional[torch.Tensor]) -> C.c_void_p:
-    return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
+def _dev_ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
 
 
 def _check_dev(t: torch.Tensor, what: str, dtype=None, numel=None):
     """A contiguous tensor on the current device (the stream the call goes to is that device's), of this type and size."""
-    if not t.is_cuda or t.device.index != torch.cuda.current_device() or not t.is_contiguous():
+    if t.get_device() < 0 or t.get_device() != torch.cuda.current_device() or not t.is_contiguous():
         raise L.NQError(L.NQ_ERR_INVALID, what + " must be a contiguous tensor on the current device")
-    if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+    if dtype is not None and t.dtype is not dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
         raise L.NQError(L.NQ_ERR_INVALID, what + " must be " + " or ".join(str(d) for d in (dtype if isinstance(dtype, tuple) else (dtype,))))
     if numel is not None and t.numel() != numel:
         raise L.NQError(L.NQ_ERR_SIZE, f"{what} has {t.numel()} values, expected {numel}")

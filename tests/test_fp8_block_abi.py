@@ -102,7 +102,7 @@ GRAD = dict(x=64, xdt=L.DT_F32, mean=64, rstd=64, gamma=64, gy=128, gydt=L.DT_F3
 @pytest.mark.parametrize("change,code,words", [
     (dict(D=0), L.NQ_ERR_INVALID, "M >= 0 and D > 0"), (dict(gydt=L.DT_I8), L.NQ_ERR_INVALID, "must be fp32 or bf16"),
     (dict(gxdt=7), L.NQ_ERR_INVALID, "must be fp32 or bf16"), (dict(dg=None), L.NQ_ERR_INVALID, "together"),
-    (dict(dg=68), L.NQ_ERR_INVALID, "16-byte"), (dict(gy=None), L.NQ_ERR_INVALID, "null pointer"),
+    (dict(dg=66), L.NQ_ERR_INVALID, "4-byte"), (dict(gy=None), L.NQ_ERR_INVALID, "null pointer"),
     (dict(mean=None), L.NQ_ERR_INVALID, "null pointer"), (dict(gx=196), L.NQ_ERR_INVALID, "16-byte"),
     (dict(gx=128, gxdt=L.DT_BF16), L.NQ_ERR_INVALID, "types agree"), (dict(gx=64, gxdt=L.DT_BF16), L.NQ_ERR_INVALID, "types agree"),
 ])
