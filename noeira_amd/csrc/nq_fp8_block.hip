@@ -20,54 +20,12 @@
 // is 2 KiB at ((R * G) + g) * 2 KiB; lane l = r + 16 c of its first KiB holds row r's k = 32 c .. 32 c + 15, of its
 // second k = 32 c + 16 .. 32 c + 31, both 16 bytes at 16 l.  A wavefront's 128-bit load is one contiguous KiB and needs
 // no exchange between lanes.  Rows behind OUT and k behind IN are zero.
-#include "nq_common.h"
+#include "nq_fp8_block.h"
 #include "nq_fp8_quant.h"
 
 namespace nq {
 
 namespace {
-
-typedef __attribute__((ext_vector_type(8))) int i32x8;
-typedef __attribute__((ext_vector_type(4))) int i32x4;
-typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
-
-// A lane's 32 bytes of an operand (16 rows x 128 k): as they are, or decoded to bf16 in four operands of 32 k each.
-// (A lane's k within an operand are the same 8 for both sides; which 8 they are does not matter to a sum.)
-template <bool EXACT>
-struct Operand;
-template <>
-struct Operand<false> {
-    i32x8 v;
-    __device__ __forceinline__ Operand(const i32x4& a, const i32x4& b) : v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]} {}
-};
-template <>
-struct Operand<true> {
-    bf16x8 v[4];
-    __device__ __forceinline__ Operand(const i32x4& a, const i32x4& b) {
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int w = s < 2 ? a[2 * s + h] : b[2 * (s - 2) + h];
-                const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
-                const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
-                v[s][4 * h] = lo[0], v[s][4 * h + 1] = lo[1], v[s][4 * h + 2] = hi[0], v[s][4 * h + 3] = hi[1];
-            }
-    }
-};
-
-// one block's sums: 16 weight rows (result rows) x 16 activation rows (result columns)
-__device__ __forceinline__ f32x4 block_sum(const Operand<false>& w, const Operand<false>& x) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, x.v, f32x4{}, 0, 0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 block_sum(const Operand<true>& w, const Operand<true>& x) {
-    f32x4 d = {};
-#pragma unroll
-    for (int s = 0; s < 4; s++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[s], x.v[s], d, 0, 0, 0);
-    return d;
-}
 
 // ---- load time ----------------------------------------------------------------------------------------------------
 
@@ -172,18 +130,6 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
-
-struct BlockParams {
-    const uint8_t* x;
-    const uint8_t* w;
-    const float* xs;
-    const float* ws;
-    const void* bias;
-    int32_t M, N, K, G;
-    int32_t tiles_m;
-    int32_t y_dtype, bias_dtype, relu;
-    SegTable seg;
-};
 
 __device__ __forceinline__ uint16_t bf16_bits(float v) {
     uint32_t bits = __float_as_uint(v);
@@ -355,6 +301,20 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
     p.M = a.M, p.N = L->out, p.K = L->in, p.G = L->groups;
     p.y_dtype = a.y_dtype, p.bias_dtype = a.bias_dtype, p.relu = a.epilogue == NQ_EPI_RELU;
     p.seg = a.seg;
+    if (fp8_block_gemm_applicable(p)) {
+        // the GEMM writes one part: a row-fused layer's parts one after the other (they begin on whole blocks)
+        for (int t = 0, r0 = 0; t < a.seg.nseg; r0 = a.seg.end[t], t++) {
+            BlockParams q = p;
+            q.w = p.w + (int64_t)(r0 / 16) * p.G * 2048;
+            q.ws = p.ws + (int64_t)(r0 / FP8_BLOCK) * p.G;
+            q.bias = !p.bias ? nullptr : reinterpret_cast<const uint8_t*>(p.bias) + (int64_t)r0 * (p.bias_dtype == NQ_DT_F32 ? 4 : 2);
+            q.N = a.seg.end[t] - r0;
+            q.seg.nseg = 1, q.seg.end[0] = q.N, q.seg.y[0] = a.seg.y[t];
+            const int32_t rc = launch_fp8_block_gemm(q, a.stream);
+            if (rc) return rc;
+        }
+        return NQ_OK;
+    }
     return launch_tile<1, 1, 4, 4>(p, a.stream);
 }
 

@@ -1,0 +1,352 @@
+// The block-scaled fp8 product for many activation rows (layout and scales: nq_fp8_block.hip):
+//     y[m, n] = epi( sum_g sx[m, g] sw[n / 128, g] * sum_{k in block g} qx[m, k] qw[n, k]  + bias[n] )
+//
+// A stage of the K loop is one block of 128 k: x tile BM x 128 B, weight tile BN x 128 B and their scales, filled straight
+// from global memory (global_load_lds) into one of NB stage buffers.  A wavefront owns TI x TJ results of 16 x 16, and its
+// channels lie in one block of 128, so its weight scale is one number per stage.
+#include <type_traits>
+
+#include "nq_fp8_block.h"
+
+namespace nq {
+
+namespace {
+
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<N, I + 1>(static_cast<F&&>(f));
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int NB, bool EXACT>
+__device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
+    constexpr int WAVES = WM * WN;
+    constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
+    constexpr int PAIRS = TJ / 2;
+    constexpr int XB = BM * 128, WB = BN * 128, SB = WAVES * 256;  // bytes of a stage: x, w, scales (256 B per wavefront)
+    constexpr int STAGE = XB + WB + SB;
+    constexpr int DX = BM / 8 / WAVES, DW = BN / 8 / WAVES;  // transfers of 1 KiB per wavefront and stage
+    constexpr int PER = DX + DW + 1;                         // ... and one of scales
+    constexpr int SW = BM / 64;                              // wavefronts that fetch x's scales; the next one fetches w's
+    static_assert(TJ % 2 == 0 && PAIRS >= 2 && BN / WN <= 128 && SW < WAVES && BM % (8 * WAVES) == 0 && BN % (16 * WAVES) == 0, "tile");
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    typedef __attribute__((address_space(3))) void lptr_t;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // ---- tile: ids are dealt round-robin to the 8 XCDs, so each XCD is given one contiguous run, and runs walk bands of 8
+    // row tiles, so that the tiles an XCD works on share their operands in its L2
+    const int nb = gridDim.x, bid = blockIdx.x;
+    const int xcd = bid % 8, lid = xcd * (nb / 8) + min(xcd, nb % 8) + bid / 8;
+    constexpr int GM = 8;
+    const int band = lid / (GM * p.tiles_n), in_band = lid - band * GM * p.tiles_n;
+    const int band_rows = min(GM, p.tiles_m - band * GM);
+    const int m0 = (band * GM + in_band % band_rows) * BM, n0 = in_band / band_rows * BN;
+
+    // ---- transfers.  x: 8 rows of 128 B per instruction, the 16-byte slots of a row permuted on the way (swz) so that the
+    // fragment reads below meet no bank twice; w: 1 KiB of operand order as it lies; scales: one float per lane.
+    auto swz = [](int row) { return (((row >> 1) & 7) + 6) & 7; };
+    const uint8_t* const xbase = p.x + (int64_t)m0 * p.K;
+    uint32_t xoff[DX];
+    int32_t xk[DX];  // where the lane's 16 bytes lie in a stage
+#pragma unroll
+    for (int t = 0; t < DX; t++) {
+        const int row = (wave * DX + t) * 8 + lane / 8;
+        xk[t] = ((lane % 8) ^ swz(row)) * 16;
+        xoff[t] = (uint32_t)(min(m0 + row, p.M - 1) - m0) * (uint32_t)p.K + xk[t];
+    }
+    const int row_tiles = (p.N + 15) / 16;
+    const uint8_t* wtile[DW / 2];  // a tile's two halves are two transfers
+#pragma unroll
+    for (int t = 0; t < DW / 2; t++) wtile[t] = p.w + (int64_t)min(n0 / 16 + wave * (DW / 2) + t, row_tiles - 1) * p.G * 2048;
+    const uint32_t woff = lane * 16;
+    const float* sbase;
+    uint32_t soff;
+    if (wave < SW) {
+        sbase = p.xs + (int64_t)m0 * p.G;
+        soff = (uint32_t)(min(m0 + wave * 64 + lane, p.M - 1) - m0) * (uint32_t)p.G * 4;
+    } else {  // (the wavefronts behind the one that is needed fetch the same again: every wavefront counts PER transfers)
+        const int b0 = n0 / 128, bl = (p.N + 127) / 128 - 1;
+        sbase = p.ws + (int64_t)b0 * p.G;
+        soff = (uint32_t)(min(b0 + min(lane, BN / 128), bl) - b0) * (uint32_t)p.G * 4;
+    }
+    // K ends inside the last block: pieces behind it come from the weight's own padding, which is zero there (a piece of
+    // 16 behind K exists in the first tile's last block, its very last)
+    const bool ragged = p.K % 128 != 0;
+    const uint8_t* const zeros = p.w + (int64_t)(p.G - 1) * 2048 + 1024 + 48 * 16;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t*)lds;
+    const int KT = p.G;
+    // transfer t of stage st into the buffer at LDS address `at`
+    auto dma = [&](auto tc, int st, uint32_t at) {
+        constexpr int t = decltype(tc)::value;
+        if constexpr (t < DX) {
+            const uint32_t m0v = at + (uint32_t)(wave * DX + t) * 1024;
+            if (ragged && st == KT - 1) {
+                const uint8_t* a = st * 128 + xk[t] < p.K ? xbase + xoff[t] + (int64_t)st * 128 : zeros;
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0v), "v"(a) : "memory");
+            } else {
+                const uint8_t* s = xbase + (int64_t)st * 128;
+                const uint32_t o = xoff[t];
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
+            }
+        } else if constexpr (t < DX + DW) {
+            constexpr int u = t - DX;
+            const uint32_t m0v = at + XB + (uint32_t)(wave * DW + u) * 1024;
+            const uint8_t* s = wtile[u / 2] + (int64_t)st * 2048 + (u & 1) * 1024;
+            const uint32_t o = woff;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
+        } else {
+            const uint32_t m0v = at + XB + WB + (uint32_t)wave * 256;
+            const float* s = sbase + st;
+            const uint32_t o = soff;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
+        }
+    };
+    // this wavefront's transfers of all but the last `keep` stages requested have landed
+    auto landed = [&](int keep) {
+        if (keep >= 2)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * PER) : "memory");
+        else if (keep == 1)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    static_assert(NB <= 4, "landed() counts to two stages");
+
+    // ---- fragments: lane l supplies bytes 32 c .. 32 c + 31 of row l % 16, c = l / 16
+    const int r = lane & 15, c = lane >> 4;
+    const uint32_t fx0 = (uint32_t)((wm * 16 * TI + r) * 128 + ((2 * c) ^ swz(r)) * 16);
+    const uint32_t fx1 = (uint32_t)((wm * 16 * TI + r) * 128 + ((2 * c + 1) ^ swz(r)) * 16);
+    const uint32_t fw = (uint32_t)(XB + wn * TJ * 2048 + lane * 16);
+    const uint32_t fs = (uint32_t)(XB + WB + (wm * 16 * TI + r) * 4), fsw = (uint32_t)(XB + WB + SW * 256 + (wn * 16 * TJ / 128) * 4);
+    i32x4 xf[TI][2], wf[2][2][2];  // token fragments; channel fragments of two pairs
+    float sx[TI], sw;
+    auto read_x = [&](int i, uint32_t at) {
+        xf[i][0] = *reinterpret_cast<const i32x4*>(lds + at + fx0 + i * 2048);
+        xf[i][1] = *reinterpret_cast<const i32x4*>(lds + at + fx1 + i * 2048);
+    };
+    auto read_w = [&](int set, int pair, uint32_t at) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                wf[set][h][e] = *reinterpret_cast<const i32x4*>(lds + at + fw + (2 * pair + h) * 2048 + e * 1024);
+    };
+    auto read_s = [&](uint32_t at) {
+#pragma unroll
+        for (int i = 0; i < TI; i++) sx[i] = *reinterpret_cast<const float*>(lds + at + fs + i * 64);
+        sw = *reinterpret_cast<const float*>(lds + at + fsw);
+    };
+
+    f32x4 acc[TI][TJ];
+#pragma unroll
+    for (int i = 0; i < TI; i++)
+#pragma unroll
+        for (int j = 0; j < TJ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // One stage, in pairs of channel fragments, token fragment by token fragment within a pair.  While a pair is multiplied
+    // the next one is read.  The last pair starts with the stage's barrier: everything of this stage has been read by then
+    // and the next one has landed, so the last pair reads the next stage's first fragments (a token fragment as soon as
+    // its last product is issued) and requests stage st + NB into the buffer just freed.  A product's four results meet
+    // their scale two products later, when the matrix core has long delivered them.
+    auto stage = [&](auto lastc, int st, uint32_t at, uint32_t next) {
+        constexpr bool LAST = decltype(lastc)::value;
+        const bool more = st + NB < KT;
+        float s[TI];
+        f32x4 part[3];
+        auto settle = [&](int q) {  // product q of the stage: pair q / (2 TI), token (q / 2) % TI, half q % 2
+            const int i = q / 2 % TI, j = 2 * (q / (2 * TI)) + q % 2;
+#pragma unroll
+            for (int t = 0; t < 4; t++) acc[i][j][t] = fmaf(part[q % 3][t], s[i], acc[i][j][t]);
+            // (here and not later: left alone, the compiler gathers the stage's multiply-adds behind its last product, with
+            // every product's result kept until then)
+            auto& a = acc;
+            asm volatile("" : "+v"(a[i][j]));
+        };
+        static_for<PAIRS>([&](auto pc) {
+            constexpr int pr = decltype(pc)::value;
+            constexpr bool END = pr == PAIRS - 1;
+            if constexpr (pr == 0) {
+#pragma unroll
+                for (int i = 0; i < TI; i++) s[i] = sx[i] * sw;
+            }
+            if constexpr (!END)
+                read_w((pr + 1) & 1, pr + 1, at);
+            else if constexpr (!LAST) {
+                landed(max(0, min(NB - 2, KT - st - 2)));
+                read_w((pr + 1) & 1, 0, next);
+                read_s(next);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const Operand<EXACT> w0(wf[pr & 1][0][0], wf[pr & 1][0][1]), w1(wf[pr & 1][1][0], wf[pr & 1][1][1]);
+            static_for<TI>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                constexpr int q = (pr * TI + i) * 2;
+                const Operand<EXACT> x(xf[i][0], xf[i][1]);
+                part[q % 3] = block_sum(w0, x);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (q >= 2) settle(q - 2);
+                if constexpr (END && !LAST) {
+                    if (more) static_for<(PER + 2 * TI - 1) / (2 * TI)>([&](auto d) {
+                        constexpr int t = 2 * i * ((PER + 2 * TI - 1) / (2 * TI)) + decltype(d)::value;
+                        if constexpr (t < PER) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
+                    });
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                part[(q + 1) % 3] = block_sum(w1, x);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (q >= 1) settle(q - 1);
+                if constexpr (END && !LAST) {
+                    read_x(i, next);
+                    if (more) static_for<(PER + 2 * TI - 1) / (2 * TI)>([&](auto d) {
+                        constexpr int t = (2 * i + 1) * ((PER + 2 * TI - 1) / (2 * TI)) + decltype(d)::value;
+                        if constexpr (t < PER) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
+                    });
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        });
+        settle(TI * TJ - 2);
+        settle(TI * TJ - 1);
+    };
+    static_assert(PAIRS % 2 == 0, "the first pair of a stage is in set 0");
+
+    for (int st = 0; st < min(NB, KT); st++) static_for<PER>([&](auto t) { dma(t, st, lds0 + st * STAGE); });
+    // (stage 0 has landed when at most the others requested are under way)
+    {
+        const int out = min(NB, KT) - 1;
+        if (out >= 3)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * PER) : "memory");
+        else if (out == 2)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
+        else if (out == 1)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+    read_w(0, 0, 0);
+    read_s(0);
+#pragma unroll
+    for (int i = 0; i < TI; i++) read_x(i, 0);
+    uint32_t at = 0;
+    for (int st = 0; st < KT - 1; st++) {
+        const uint32_t next = at == (NB - 1) * STAGE ? 0 : at + STAGE;
+        stage(std::false_type{}, st, at, next);
+        at = next;
+    }
+    stage(std::true_type{}, KT - 1, at, 0);
+    __syncthreads();  // (nothing is under way: the last requests were waited for a stage ago)
+
+    // ---- epilogue: a lane holds token 16 i + r and channels 16 j + 4 c .. + 3.  A wavefront stages 32 tokens at a time in
+    // LDS of its own and writes them as 128-bit stores, whole rows of its channels.
+    constexpr int ES = EXACT ? 4 : 2, CH = 16 * TJ, ROWB = CH * ES + 16;
+    static_assert(WAVES * 32 * ROWB <= NB * STAGE, "the epilogue stages in the stage buffers");
+    uint8_t* const stg = lds + wave * 32 * ROWB;
+    const int wm0 = m0 + wm * 16 * TI, wn0 = n0 + wn * CH;
+    uint8_t* const y = reinterpret_cast<uint8_t*>(p.seg.y[0]);
+    const bool whole = wn0 + CH <= p.N && p.N % (16 / ES) == 0 && ((uintptr_t)y & 15) == 0;
+#pragma unroll
+    for (int ip = 0; ip < TI; ip += 2) {
+#pragma unroll
+        for (int j = 0; j < TJ; j++) {
+            float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.bias) {
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int n = min(wn0 + 16 * j + 4 * c + t, p.N - 1);
+                    b[t] = p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[n]
+                                                     : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[n] << 16);
+                }
+            }
+#pragma unroll
+            for (int ii = 0; ii < 2; ii++) {
+                f32x4 z;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    z[t] = acc[ip + ii][j][t] + b[t];
+                    if (p.relu) z[t] = z[t] > 0.0f ? z[t] : 0.0f;
+                }
+                uint8_t* dst = stg + (16 * ii + r) * ROWB + (16 * j + 4 * c) * ES;
+                if constexpr (EXACT)
+                    *reinterpret_cast<f32x4*>(dst) = z;
+                else
+                    *reinterpret_cast<bf16x4*>(dst) = __builtin_convertvector(z, bf16x4);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        constexpr int LPR = CH * ES / 16, RPI = 64 / LPR;  // lanes per row, rows per instruction
+#pragma unroll
+        for (int t = 0; t < 32 / RPI; t++) {
+            const int row = t * RPI + lane / LPR, c16 = lane % LPR;
+            const i32x4 v = *reinterpret_cast<const i32x4*>(stg + row * ROWB + c16 * 16);
+            const int m = wm0 + 16 * ip + row, n = wn0 + c16 * (16 / ES);
+            if (m >= p.M) continue;
+            if (whole) {
+                *reinterpret_cast<i32x4*>(y + ((int64_t)m * p.N + n) * ES) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16 / ES; e++) {
+                    if (n + e >= p.N) break;
+                    if constexpr (EXACT)
+                        reinterpret_cast<int32_t*>(y)[(int64_t)m * p.N + n + e] = v[e];
+                    else
+                        reinterpret_cast<uint16_t*>(y)[(int64_t)m * p.N + n + e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+// 256 x 256 on eight wavefronts (64 x 128 each, two per SIMD), two stage buffers
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_block_gemm_kernel(const BlockParams p) {
+    block_gemm_body<256, 256, 4, 2, 2, false>(p);
+}
+// 128 x 128 on four wavefronts (64 x 64 each), four stage buffers
+template <bool EXACT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void fp8_block_gemm128_kernel(const BlockParams p) {
+    block_gemm_body<128, 128, 2, 2, 4, EXACT>(p);
+}
+
+constexpr size_t lds_bytes(int bm, int bn, int waves, int nb) { return (size_t)nb * ((bm + bn) * 128 + waves * 256); }
+
+template <typename K>
+int32_t launch(K kernel, LdsAttrOnce& attr, BlockParams p, int bm, int bn, int waves, int nb, hipStream_t s) {
+    p.tiles_m = (p.M - 1) / bm + 1, p.tiles_n = (p.N - 1) / bn + 1;
+    const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
+    if (grid * 64 > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
+    const size_t lds = lds_bytes(bm, bn, waves, nb);
+    NQ_HIP(set_max_lds_once(attr, reinterpret_cast<const void*>(kernel), lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), lds, s, p);
+    NQ_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+}  // namespace
+
+bool fp8_block_gemm_applicable(const BlockParams& p) {
+    // 32-bit offsets from a tile's base
+    return p.M > 64 && (int64_t)p.K * 256 < ((int64_t)1 << 32);
+}
+
+double fp8_block_gemm_estimate_us(const BlockParams& p) { return p.M > 64 ? 0.0 : 1e9; }
+
+int32_t launch_fp8_block_gemm(const BlockParams& p, hipStream_t s) {
+    static LdsAttrOnce attr[3];
+    if (p.y_dtype == NQ_DT_F32) return launch(fp8_block_gemm128_kernel<true>, attr[0], p, 128, 128, 4, 4, s);
+    if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) < 128) return launch(fp8_block_gemm128_kernel<false>, attr[1], p, 128, 128, 4, 4, s);
+    return launch(fp8_block_gemm_kernel, attr[2], p, 256, 256, 8, 2, s);
+}
+
+}  // namespace nq
