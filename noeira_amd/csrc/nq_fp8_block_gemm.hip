@@ -25,14 +25,14 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     constexpr int WAVES = WM * WN;
     constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
     constexpr int PAIRS = TJ / 2;
-    constexpr int XB = BM * 128, WB = BN * 128, SB = WAVES * 256;  // bytes of a stage: x, w, scales (256 B per wavefront)
-    constexpr int STAGE = XB + WB + SB;
-    constexpr int DX = BM / 8 / WAVES, DW = BN / 8 / WAVES;  // transfers of 1 KiB per wavefront and stage
-    constexpr int PER = DX + DW + 1;                         // ... and one of scales
-    constexpr int SW = BM / 64;                              // wavefronts that fetch x's scales; the next one fetches w's
-    static_assert(TJ % 2 == 0 && PAIRS >= 2 && BN / WN <= 128 && SW < WAVES && BM % (8 * WAVES) == 0 && BN % (16 * WAVES) == 0, "tile");
+    constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB;  // bytes of a stage
+    constexpr int DX = BM / 8 / WAVES, DW = BN / 8 / WAVES;       // transfers of 1 KiB per wavefront and stage
+    constexpr int SW = BM / 64;                                   // wavefronts that fetch x's scales; the next one fetches w's
+    constexpr int CHUNK_BYTES = BM * 16 + 256;                    // scales of four stages: [BM][4], then [BN / 128][4]
+    static_assert(TJ % 2 == 0 && PAIRS % 2 == 0 && BN / WN <= 128 && SW < WAVES && BM % (8 * WAVES) == 0 && BN % (16 * WAVES) == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     typedef __attribute__((address_space(3))) void lptr_t;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t*)lds;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -63,21 +63,25 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
 #pragma unroll
     for (int t = 0; t < DW / 2; t++) wtile[t] = p.w + (int64_t)min(n0 / 16 + wave * (DW / 2) + t, row_tiles - 1) * p.G * 2048;
     const uint32_t woff = lane * 16;
-    const float* sbase;
-    uint32_t soff;
-    if (wave < SW) {
-        sbase = p.xs + (int64_t)m0 * p.G;
-        soff = (uint32_t)(min(m0 + wave * 64 + lane, p.M - 1) - m0) * (uint32_t)p.G * 4;
-    } else {  // (the wavefronts behind the one that is needed fetch the same again: every wavefront counts PER transfers)
-        const int b0 = n0 / 128, bl = (p.N + 127) / 128 - 1;
-        sbase = p.ws + (int64_t)b0 * p.G;
-        soff = (uint32_t)(min(b0 + min(lane, BN / 128), bl) - b0) * (uint32_t)p.G * 4;
-    }
+    // Scales come four stages at a time (a row's four are 16 adjacent bytes; one at a time, 64 rows to an instruction,
+    // they cost 3 - 6 % of the call), in three buffers taken in turn: with stage s goes a quarter of the chunk after its
+    // own, which has landed with it, a stage ahead of its first use at the latest, and whose buffer held the chunk
+    // before stage s's: the stage being multiplied is at most NB <= 4 stages behind s.
+    const bool sx_wave = wave < SW, scaling = wave <= SW;
+    const float* const sbase = sx_wave ? p.xs + (int64_t)m0 * p.G : p.ws + (int64_t)(n0 / 128) * p.G;
+    const int srow_end = sx_wave ? p.M - m0 : (p.N + 127) / 128 - n0 / 128;
+    const uint32_t scales0 = NB * STAGE;
+    auto scale_dma = [&](int chunk, int quarter) {
+        const int row = sx_wave ? (quarter * SW + wave) * 16 + lane / 4 : lane / 4;
+        const uint32_t o = ((uint32_t)min(row, srow_end - 1) * (uint32_t)p.G + (uint32_t)min(4 * chunk + lane % 4, p.G - 1)) * 4;
+        const uint32_t m0v = lds0 + scales0 + (uint32_t)(chunk % 3) * CHUNK_BYTES + (sx_wave ? (uint32_t)(quarter * SW + wave) * 256 : BM * 16);
+        const float* s = sbase;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
+    };
     // K ends inside the last block: pieces behind it come from the weight's own padding, which is zero there (a piece of
     // 16 behind K exists in the first tile's last block, its very last)
     const bool ragged = p.K % 128 != 0;
     const uint8_t* const zeros = p.w + (int64_t)(p.G - 1) * 2048 + 1024 + 48 * 16;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t*)lds;
     const int KT = p.G;
     // transfer t of stage st into the buffer at LDS address `at`
     auto dma = [&](auto tc, int st, uint32_t at) {
@@ -92,38 +96,43 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 const uint32_t o = xoff[t];
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
             }
-        } else if constexpr (t < DX + DW) {
+        } else {
             constexpr int u = t - DX;
             const uint32_t m0v = at + XB + (uint32_t)(wave * DW + u) * 1024;
             const uint8_t* s = wtile[u / 2] + (int64_t)st * 2048 + (u & 1) * 1024;
             const uint32_t o = woff;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
-        } else {
-            const uint32_t m0v = at + XB + WB + (uint32_t)wave * 256;
-            const float* s = sbase + st;
-            const uint32_t o = soff;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
         }
     };
-    // this wavefront's transfers of all but the last `keep` stages requested have landed
-    auto landed = [&](int keep) {
-        if (keep >= 2)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * PER) : "memory");
-        else if (keep == 1)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER) : "memory");
+    // Everything a wavefront has requested has landed but for its last `keep` stages (the scaling wavefronts have one
+    // transfer more per stage: transfers land in the order of issue)
+    auto wait_all_but = [&](auto kc) {
+        constexpr int keep = decltype(kc)::value;
+        if (keep > 0 && scaling)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep * (DX + DW + 1)) : "memory");
         else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep * (DX + DW)) : "memory");
+    };
+    auto landed = [&](int keep) {
+        if (NB >= 4 && keep >= 3)
+            wait_all_but(std::integral_constant<int, NB >= 4 ? 3 : 0>{});
+        else if (NB >= 3 && keep >= 2)
+            wait_all_but(std::integral_constant<int, NB >= 3 ? 2 : 0>{});
+        else if (keep >= 1)
+            wait_all_but(std::integral_constant<int, 1>{});
+        else
+            wait_all_but(std::integral_constant<int, 0>{});
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    static_assert(NB <= 4, "landed() counts to two stages");
+    static_assert(NB <= 4 && NB >= 2, "landed() counts to three stages, three chunk buffers serve four");
 
     // ---- fragments: lane l supplies bytes 32 c .. 32 c + 31 of row l % 16, c = l / 16
     const int r = lane & 15, c = lane >> 4;
     const uint32_t fx0 = (uint32_t)((wm * 16 * TI + r) * 128 + ((2 * c) ^ swz(r)) * 16);
     const uint32_t fx1 = (uint32_t)((wm * 16 * TI + r) * 128 + ((2 * c + 1) ^ swz(r)) * 16);
     const uint32_t fw = (uint32_t)(XB + wn * TJ * 2048 + lane * 16);
-    const uint32_t fs = (uint32_t)(XB + WB + (wm * 16 * TI + r) * 4), fsw = (uint32_t)(XB + WB + SW * 256 + (wn * 16 * TJ / 128) * 4);
+    const uint32_t fs = scales0 + (wm * 16 * TI + r) * 16, fsw = scales0 + BM * 16 + (wn * 16 * TJ / 128) * 16;
     i32x4 xf[TI][2], wf[2][2][2];  // token fragments; channel fragments of two pairs
     float sx[TI], sw;
     auto read_x = [&](int i, uint32_t at) {
@@ -137,10 +146,11 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             for (int e = 0; e < 2; e++)
                 wf[set][h][e] = *reinterpret_cast<const i32x4*>(lds + at + fw + (2 * pair + h) * 2048 + e * 1024);
     };
-    auto read_s = [&](uint32_t at) {
+    auto read_s = [&](int st) {
+        const uint32_t o = (uint32_t)(st / 4 % 3) * CHUNK_BYTES + (uint32_t)(st % 4) * 4;
 #pragma unroll
-        for (int i = 0; i < TI; i++) sx[i] = *reinterpret_cast<const float*>(lds + at + fs + i * 64);
-        sw = *reinterpret_cast<const float*>(lds + at + fsw);
+        for (int i = 0; i < TI; i++) sx[i] = *reinterpret_cast<const float*>(lds + o + fs + i * 256);
+        sw = *reinterpret_cast<const float*>(lds + o + fsw);
     };
 
     f32x4 acc[TI][TJ];
@@ -156,6 +166,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     // their scale two products later, when the matrix core has long delivered them.
     auto stage = [&](auto lastc, int st, uint32_t at, uint32_t next) {
         constexpr bool LAST = decltype(lastc)::value;
+        constexpr int SLOT = (DX + DW + 2 * TI - 1) / (2 * TI);  // transfers behind a product of the last pair
         const bool more = st + NB < KT;
         float s[TI];
         f32x4 part[3];
@@ -180,7 +191,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             else if constexpr (!LAST) {
                 landed(max(0, min(NB - 2, KT - st - 2)));
                 read_w((pr + 1) & 1, 0, next);
-                read_s(next);
+                read_s(st + 1);
             }
             __builtin_amdgcn_sched_barrier(0);
             const Operand<EXACT> w0(wf[pr & 1][0][0], wf[pr & 1][0][1]), w1(wf[pr & 1][1][0], wf[pr & 1][1][1]);
@@ -192,9 +203,9 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (q >= 2) settle(q - 2);
                 if constexpr (END && !LAST) {
-                    if (more) static_for<(PER + 2 * TI - 1) / (2 * TI)>([&](auto d) {
-                        constexpr int t = 2 * i * ((PER + 2 * TI - 1) / (2 * TI)) + decltype(d)::value;
-                        if constexpr (t < PER) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
+                    if (more) static_for<SLOT>([&](auto d) {
+                        constexpr int t = 2 * i * SLOT + decltype(d)::value;
+                        if constexpr (t < DX + DW) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
                     });
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -203,10 +214,12 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 if constexpr (q >= 1) settle(q - 1);
                 if constexpr (END && !LAST) {
                     read_x(i, next);
-                    if (more) static_for<(PER + 2 * TI - 1) / (2 * TI)>([&](auto d) {
-                        constexpr int t = (2 * i + 1) * ((PER + 2 * TI - 1) / (2 * TI)) + decltype(d)::value;
-                        if constexpr (t < PER) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
+                    if (more) static_for<SLOT>([&](auto d) {
+                        constexpr int t = (2 * i + 1) * SLOT + decltype(d)::value;
+                        if constexpr (t < DX + DW) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
                     });
+                    if constexpr (i == TI - 1)
+                        if (more && scaling) scale_dma((st + NB) / 4 + 1, (st + NB) % 4);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             });
@@ -214,23 +227,14 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
         settle(TI * TJ - 2);
         settle(TI * TJ - 1);
     };
-    static_assert(PAIRS % 2 == 0, "the first pair of a stage is in set 0");
 
-    for (int st = 0; st < min(NB, KT); st++) static_for<PER>([&](auto t) { dma(t, st, lds0 + st * STAGE); });
-    // (stage 0 has landed when at most the others requested are under way)
-    {
-        const int out = min(NB, KT) - 1;
-        if (out >= 3)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * PER) : "memory");
-        else if (out == 2)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
-        else if (out == 1)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+    if (scaling)
+        for (int q = 0; q < 4; q++) scale_dma(0, q);
+    for (int st = 0; st < min(NB, KT); st++) {
+        static_for<DX + DW>([&](auto t) { dma(t, st, lds0 + st * STAGE); });
+        if (scaling) scale_dma(st / 4 + 1, st % 4);
     }
+    landed(min(NB, KT) - 1);
     read_w(0, 0, 0);
     read_s(0);
 #pragma unroll
@@ -309,26 +313,24 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     }
 }
 
-// 256 x 256 on eight wavefronts (64 x 128 each, two per SIMD), two stage buffers
+template <int BM, int BN, int NB>
+constexpr size_t lds_bytes() { return (size_t)NB * (BM + BN) * 128 + 3 * (BM * 16 + 256); }
+
+// eight wavefronts, 4 x 2, two per SIMD
+template <int BM, int BN, int NB, bool EXACT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_block_gemm_kernel(const BlockParams p) {
-    block_gemm_body<256, 256, 4, 2, 2, false>(p);
-}
-// 128 x 128 on four wavefronts (64 x 64 each), four stage buffers
-template <bool EXACT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void fp8_block_gemm128_kernel(const BlockParams p) {
-    block_gemm_body<128, 128, 2, 2, 4, EXACT>(p);
+    block_gemm_body<BM, BN, 4, 2, NB, EXACT>(p);
 }
 
-constexpr size_t lds_bytes(int bm, int bn, int waves, int nb) { return (size_t)nb * ((bm + bn) * 128 + waves * 256); }
-
-template <typename K>
-int32_t launch(K kernel, LdsAttrOnce& attr, BlockParams p, int bm, int bn, int waves, int nb, hipStream_t s) {
-    p.tiles_m = (p.M - 1) / bm + 1, p.tiles_n = (p.N - 1) / bn + 1;
+template <int BM, int BN, int NB, bool EXACT>
+int32_t launch(BlockParams p, hipStream_t s) {
+    static LdsAttrOnce attr;
+    p.tiles_m = (p.M - 1) / BM + 1, p.tiles_n = (p.N - 1) / BN + 1;
     const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
-    if (grid * 64 > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
-    const size_t lds = lds_bytes(bm, bn, waves, nb);
-    NQ_HIP(set_max_lds_once(attr, reinterpret_cast<const void*>(kernel), lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), lds, s, p);
+    if (grid * 512 > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
+    const void* kernel = reinterpret_cast<const void*>(&fp8_block_gemm_kernel<BM, BN, NB, EXACT>);
+    NQ_HIP(set_max_lds_once(attr, kernel, lds_bytes<BM, BN, NB>()));
+    hipLaunchKernelGGL((fp8_block_gemm_kernel<BM, BN, NB, EXACT>), dim3((unsigned)grid), dim3(512), (lds_bytes<BM, BN, NB>()), s, p);
     NQ_HIP(hipGetLastError());
     return NQ_OK;
 }
@@ -343,10 +345,9 @@ bool fp8_block_gemm_applicable(const BlockParams& p) {
 double fp8_block_gemm_estimate_us(const BlockParams& p) { return p.M > 64 ? 0.0 : 1e9; }
 
 int32_t launch_fp8_block_gemm(const BlockParams& p, hipStream_t s) {
-    static LdsAttrOnce attr[3];
-    if (p.y_dtype == NQ_DT_F32) return launch(fp8_block_gemm128_kernel<true>, attr[0], p, 128, 128, 4, 4, s);
-    if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) < 128) return launch(fp8_block_gemm128_kernel<false>, attr[1], p, 128, 128, 4, 4, s);
-    return launch(fp8_block_gemm_kernel, attr[2], p, 256, 256, 8, 2, s);
+    if (p.y_dtype == NQ_DT_F32) return launch<128, 128, 4, true>(p, s);
+    if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) < 128) return launch<128, 128, 4, false>(p, s);
+    return launch<256, 256, 2, false>(p, s);
 }
 
 }  // namespace nq
