@@ -17,9 +17,11 @@
 // multiplies the codes.
 //
 // Weight layout.  The codes are kept only in the matrix core's operand order: tile (R, g) = rows 16 R .., k = 128 g ..
-// is 2 KiB at ((R * G) + g) * 2 KiB; lane l = r + 16 c of its first KiB holds row r's k = 32 c .. 32 c + 15, of its
-// second k = 32 c + 16 .. 32 c + 31, both 16 bytes at 16 l.  A wavefront's 128-bit load is one contiguous KiB and needs
-// no exchange between lanes.  Rows behind OUT and k behind IN are zero.
+// is 2 KiB at ((R * G) + g) * 2 KiB; lane l = r + 16 c of its first KiB holds row r's k = 16 c .. 16 c + 15, of its
+// second k = 64 + 16 c .. 64 + 16 c + 15, both 16 bytes at 16 l.  A wavefront's 128-bit load is one contiguous KiB and
+// needs no exchange between lanes.  (Which of the 128 k a lane multiplies is free as long as both operands agree; with
+// these a lane's loads of the row-ordered activations are 64 adjacent bytes per row and instruction.)  Rows behind
+// OUT and k behind IN are zero.
 #include "nq_fp8_block.h"
 #include "nq_fp8_quant.h"
 
@@ -41,7 +43,7 @@ __global__ __launch_bounds__(256) void fp8_block_repack_kernel(const uint8_t* __
     const int lane = (int)(t & 63), half = (int)(t >> 6) & 1;
     const int64_t tile = t >> 7;
     const int64_t row = tile / G * 16 + (lane & 15);
-    const int64_t k0 = tile % G * 128 + 32 * (lane >> 4) + 16 * half;
+    const int64_t k0 = tile % G * 128 + 64 * half + 16 * (lane >> 4);
     uint32_t w[4] = {0, 0, 0, 0};
     if (row < trows) {
 #pragma unroll
@@ -66,7 +68,7 @@ __global__ __launch_bounds__(256) void fp8_block_dequantize_kernel(const uint8_t
     const int32_t pieces = K / 16;
     if (t >= (int64_t)N * pieces) return;
     const int64_t n = t / pieces;
-    const int32_t k = (int32_t)(t % pieces) * 16, g = k / 128, c = k / 32 % 4, half = k / 16 % 2;
+    const int32_t k = (int32_t)(t % pieces) * 16, g = k / 128, c = k / 16 % 4, half = k / 64 % 2;
     const uint4 v = *reinterpret_cast<const uint4*>(tiles + (n / 16 * G + g) * 2048 + half * 1024 + (n % 16 + 16 * c) * 16);
     const float s = ws[n / 128 * G + g];
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -131,12 +133,6 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void
 
 // ---- the product --------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint16_t bf16_bits(float v) {
-    uint32_t bits = __float_as_uint(v);
-    if ((bits & 0x7FFFFFFFu) > 0x7F800000u) return 0x7FC0;
-    return (uint16_t)((bits + 0x7FFFu + ((bits >> 16) & 1u)) >> 16);
-}
-
 // MT x NT MFMA tiles of 16 x 16 per workgroup, the blocks of K dealt over KW wavefronts, whose sums meet in LDS in
 // wavefront order (bit-repeatable).  U: blocks requested together.
 template <int MT, int NT, int KW, int U, bool EXACT>
@@ -184,7 +180,7 @@ __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockPara
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     // (K is a multiple of 16: a piece lies in the row or behind it, and what lies behind counts as zero)
-                    const int k = 128 * g + 32 * c + 16 * e;
+                    const int k = 128 * g + 64 * e + 16 * c;
                     const i32x4 v = *reinterpret_cast<const i32x4*>(p.x + mrow[i] * p.K + (k < p.K ? k : 0));
                     xv[u][i][e] = k < p.K ? v : i32x4{0, 0, 0, 0};
                 }
@@ -214,24 +210,50 @@ __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockPara
 #pragma unroll
         for (int j = 0; j < NT; j++) *reinterpret_cast<f32x4*>(&part[wave][16 * i + r][16 * j + 4 * c]) = acc[i][j];
     __syncthreads();
-    for (int o = threadIdx.x; o < ROWS * CH; o += 64 * KW) {
-        const int row = o / CH, ch = o % CH;
+    // four channels of a row per thread, a part's boundary never among them (parts begin on a multiple of 128)
+    for (int o = threadIdx.x; o < ROWS * CH / 4; o += 64 * KW) {
+        const int row = o / (CH / 4), ch = o % (CH / 4) * 4;
         const int m = m0 + row, n = n0 + ch;
         if (m >= p.M || n >= p.N) continue;
-        float z = part[0][row][ch];
+        f32x4 z = *reinterpret_cast<const f32x4*>(&part[0][row][ch]);
 #pragma unroll
-        for (int w = 1; w < KW; w++) z += part[w][row][ch];
-        if (p.bias)
-            z += p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[n]
-                                           : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[n] << 16);
-        if (p.relu) z = z > 0.0f ? z : 0.0f;
+        for (int w = 1; w < KW; w++) z += *reinterpret_cast<const f32x4*>(&part[w][row][ch]);
+        if (p.bias) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const int nn = min(n + t, p.N - 1);
+                z[t] += p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[nn]
+                                                  : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[nn] << 16);
+            }
+        }
+        if (p.relu) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) z[t] = z[t] > 0.0f ? z[t] : 0.0f;
+        }
         void* y;
         int width, col;
         seg_lookup(p.seg, n, y, width, col);
-        if (p.y_dtype == NQ_DT_F32)
-            reinterpret_cast<float*>(y)[(int64_t)m * width + col] = z;
-        else
-            reinterpret_cast<uint16_t*>(y)[(int64_t)m * width + col] = bf16_bits(z);
+        const int64_t at = (int64_t)m * width + col;
+        if (EXACT) {
+            float* q = reinterpret_cast<float*>(y) + at;
+            if (((uintptr_t)q & 15) == 0 && n + 4 <= p.N) {
+                *reinterpret_cast<f32x4*>(q) = z;
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    if (n + t < p.N) q[t] = z[t];
+            }
+        } else {
+            const bf16x4 b = __builtin_convertvector(z, bf16x4);
+            __bf16* q = reinterpret_cast<__bf16*>(y) + at;
+            if (((uintptr_t)q & 7) == 0 && n + 4 <= p.N) {
+                *reinterpret_cast<bf16x4*>(q) = b;
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+                    if (n + t < p.N) q[t] = b[t];
+            }
+        }
     }
 }
 

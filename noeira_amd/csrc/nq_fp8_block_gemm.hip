@@ -30,6 +30,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     constexpr int SW = BM / 64;                                   // wavefronts that fetch x's scales; the next one fetches w's
     constexpr int CHUNK_BYTES = BM * 16 + 256;                    // scales of four stages: [BM][4], then [BN / 128][4]
     static_assert(TJ % 2 == 0 && PAIRS % 2 == 0 && BN / WN <= 128 && SW < WAVES && BM % (8 * WAVES) == 0 && BN % (16 * WAVES) == 0, "tile");
+    static_assert(NB >= 2 && NB <= 4 && (NB > 2 || PAIRS >= 3), "the places of the transfers; three buffers of scales");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     typedef __attribute__((address_space(3))) void lptr_t;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t*)lds;
@@ -104,33 +105,24 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
         }
     };
-    // Everything a wavefront has requested has landed but for its last `keep` stages (the scaling wavefronts have one
-    // transfer more per stage: transfers land in the order of issue)
-    auto wait_all_but = [&](auto kc) {
-        constexpr int keep = decltype(kc)::value;
-        if (keep > 0 && scaling)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep * (DX + DW + 1)) : "memory");
+    // Everything this wavefront has requested has landed but for the last `keep` transfers and `scales` of scales (which
+    // only the scaling wavefronts have; transfers land in the order of issue), and so for all wavefronts behind the barrier.
+    auto landed = [&](auto keepc, auto scalesc) {
+        constexpr int keep = decltype(keepc)::value, scales = decltype(scalesc)::value;
+        if (scales > 0 && scaling)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep + scales) : "memory");
         else
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep * (DX + DW)) : "memory");
-    };
-    auto landed = [&](int keep) {
-        if (NB >= 4 && keep >= 3)
-            wait_all_but(std::integral_constant<int, NB >= 4 ? 3 : 0>{});
-        else if (NB >= 3 && keep >= 2)
-            wait_all_but(std::integral_constant<int, NB >= 3 ? 2 : 0>{});
-        else if (keep >= 1)
-            wait_all_but(std::integral_constant<int, 1>{});
-        else
-            wait_all_but(std::integral_constant<int, 0>{});
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    static_assert(NB <= 4 && NB >= 2, "landed() counts to three stages, three chunk buffers serve four");
+    using std::integral_constant;
+    using none = integral_constant<int, 0>;
 
-    // ---- fragments: lane l supplies bytes 32 c .. 32 c + 31 of row l % 16, c = l / 16
+    // ---- fragments: lane l supplies bytes 16 c .. 16 c + 15 of both halves of row l % 16, c = l / 16
     const int r = lane & 15, c = lane >> 4;
-    const uint32_t fx0 = (uint32_t)((wm * 16 * TI + r) * 128 + ((2 * c) ^ swz(r)) * 16);
-    const uint32_t fx1 = (uint32_t)((wm * 16 * TI + r) * 128 + ((2 * c + 1) ^ swz(r)) * 16);
+    const uint32_t fx0 = (uint32_t)((wm * 16 * TI + r) * 128 + (c ^ swz(r)) * 16);
+    const uint32_t fx1 = (uint32_t)((wm * 16 * TI + r) * 128 + ((4 + c) ^ swz(r)) * 16);
     const uint32_t fw = (uint32_t)(XB + wn * TJ * 2048 + lane * 16);
     const uint32_t fs = scales0 + (wm * 16 * TI + r) * 16, fsw = scales0 + BM * 16 + (wn * 16 * TJ / 128) * 16;
     i32x4 xf[TI][2], wf[2][2][2];  // token fragments; channel fragments of two pairs
@@ -161,13 +153,21 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
 
     // One stage, in pairs of channel fragments, token fragment by token fragment within a pair.  While a pair is multiplied
     // the next one is read.  The last pair starts with the stage's barrier: everything of this stage has been read by then
-    // and the next one has landed, so the last pair reads the next stage's first fragments (a token fragment as soon as
-    // its last product is issued) and requests stage st + NB into the buffer just freed.  A product's four results meet
-    // their scale two products later, when the matrix core has long delivered them.
-    auto stage = [&](auto lastc, int st, uint32_t at, uint32_t next) {
+    // and the next one has landed, so the last pair reads the next stage's first fragments, a token fragment as soon as
+    // its last product is issued.  A product's four results meet their scale two products later, when the matrix core has
+    // long delivered them.
+    //
+    // The transfers stand between the products, spread out: the CU's address unit takes about 22 cycles for each, and a
+    // wavefront that finds it busy waits with its products behind it (all of a stage's in its last pair: XXX).  With three
+    // buffers and more, stage st requests stage st + NB - 1 into the buffer that the last barrier freed.  With two, that
+    // would leave a stage's last transfers no time to land; there the two halves of the buffer are freed one after the
+    // other: the x half by a barrier behind the first pair (the token fragments are in registers by then), refilled during
+    // the middle pairs, the w half by the stage's own barrier, refilled during its last pair and the next one's first.
+    constexpr int Q = TI * TJ, QB = Q - 2 * TI;  // products of a stage; the first one behind its barrier
+    constexpr int T = DX + DW;
+    auto stage = [&](auto lastc, int st, uint32_t at, uint32_t next, uint32_t prev) {
         constexpr bool LAST = decltype(lastc)::value;
-        constexpr int SLOT = (DX + DW + 2 * TI - 1) / (2 * TI);  // transfers behind a product of the last pair
-        const bool more = st + NB < KT;
+        const bool more = st + (NB >= 3 ? NB - 1 : 2) < KT;
         float s[TI];
         f32x4 part[3];
         auto settle = [&](int q) {  // product q of the stage: pair q / (2 TI), token (q / 2) % TI, half q % 2
@@ -179,6 +179,38 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             auto& a = acc;
             asm volatile("" : "+v"(a[i][j]));
         };
+        auto transfers = [&](auto qc) {  // behind product q
+            constexpr int q = decltype(qc)::value;
+            auto some = [&](auto firstc, auto endc, int to, uint32_t buffer) {
+                constexpr int first = decltype(firstc)::value, end = decltype(endc)::value;
+                static_for<end - first>([&](auto d) { dma(integral_constant<int, first + decltype(d)::value>{}, to, lds0 + buffer); });
+            };
+            if constexpr (LAST) {
+            } else if constexpr (NB >= 3) {
+                constexpr int from = q * T / Q, to = (q + 1) * T / Q;
+                if constexpr (to > from)
+                    if (more) some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + NB - 1, prev);
+                if constexpr (q == Q - 1)
+                    if (more && scaling) scale_dma((st + NB - 1) / 4 + 1, (st + NB - 1) % 4);
+            } else {
+                constexpr int HALF = DW / 2, FIRST = 2 * TI;  // products of the first pair, and of the last
+                if constexpr (q < FIRST) {
+                    constexpr int from = DX + HALF + q * (DW - HALF) / FIRST, to = DX + HALF + (q + 1) * (DW - HALF) / FIRST;
+                    if constexpr (to > from)
+                        if (st > 0) some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + 1, next);
+                } else if constexpr (q < QB) {
+                    constexpr int from = (q - FIRST) * DX / (QB - FIRST), to = (q - FIRST + 1) * DX / (QB - FIRST);
+                    if constexpr (to > from)
+                        if (more) some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + 2, at);
+                    if constexpr (q == QB - 1)
+                        if (more && scaling) scale_dma((st + 2) / 4 + 1, (st + 2) % 4);
+                } else {
+                    constexpr int from = DX + (q - QB) * HALF / FIRST, to = DX + (q - QB + 1) * HALF / FIRST;
+                    if constexpr (to > from)
+                        if (more) some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + 2, at);
+                }
+            }
+        };
         static_for<PAIRS>([&](auto pc) {
             constexpr int pr = decltype(pc)::value;
             constexpr bool END = pr == PAIRS - 1;
@@ -186,10 +218,30 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
 #pragma unroll
                 for (int i = 0; i < TI; i++) s[i] = sx[i] * sw;
             }
+            if constexpr (NB == 2 && pr == 1 && !LAST) {
+                if (more) {
+                    asm volatile("" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+            }
             if constexpr (!END)
                 read_w((pr + 1) & 1, pr + 1, at);
             else if constexpr (!LAST) {
-                landed(max(0, min(NB - 2, KT - st - 2)));
+                // under way may be: what this stage has requested so far, and (four buffers) the stage after the next one
+                if constexpr (NB >= 3) {
+                    if (more)
+                        landed(integral_constant<int, (NB - 3) * T + QB * T / Q>{}, integral_constant<int, NB - 3>{});
+                    else if (NB == 4 && st + 2 < KT)
+                        landed(integral_constant<int, T>{}, integral_constant<int, 1>{});
+                    else
+                        landed(none{}, none{});
+                } else {
+                    if (more)
+                        landed(integral_constant<int, DX>{}, integral_constant<int, 1>{});
+                    else
+                        landed(none{}, none{});
+                }
                 read_w((pr + 1) & 1, 0, next);
                 read_s(st + 1);
             }
@@ -202,50 +254,42 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 part[q % 3] = block_sum(w0, x);
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (q >= 2) settle(q - 2);
-                if constexpr (END && !LAST) {
-                    if (more) static_for<SLOT>([&](auto d) {
-                        constexpr int t = 2 * i * SLOT + decltype(d)::value;
-                        if constexpr (t < DX + DW) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
-                    });
-                }
+                transfers(integral_constant<int, q>{});
                 __builtin_amdgcn_sched_barrier(0);
                 part[(q + 1) % 3] = block_sum(w1, x);
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (q >= 1) settle(q - 1);
-                if constexpr (END && !LAST) {
-                    read_x(i, next);
-                    if (more) static_for<SLOT>([&](auto d) {
-                        constexpr int t = (2 * i + 1) * SLOT + decltype(d)::value;
-                        if constexpr (t < DX + DW) dma(std::integral_constant<int, t>{}, st + NB, lds0 + at);
-                    });
-                    if constexpr (i == TI - 1)
-                        if (more && scaling) scale_dma((st + NB) / 4 + 1, (st + NB) % 4);
-                }
+                if constexpr (END && !LAST) read_x(i, next);
+                transfers(integral_constant<int, q + 1>{});
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
-        settle(TI * TJ - 2);
-        settle(TI * TJ - 1);
+        settle(Q - 2);
+        settle(Q - 1);
     };
 
+    constexpr int AHEAD = NB >= 3 ? NB - 1 : 2;  // stages requested before the first
     if (scaling)
         for (int q = 0; q < 4; q++) scale_dma(0, q);
-    for (int st = 0; st < min(NB, KT); st++) {
-        static_for<DX + DW>([&](auto t) { dma(t, st, lds0 + st * STAGE); });
+    for (int st = 0; st < min(AHEAD, KT); st++) {
+        static_for<T>([&](auto t) { dma(t, st, lds0 + st * STAGE); });
         if (scaling) scale_dma(st / 4 + 1, st % 4);
     }
-    landed(min(NB, KT) - 1);
+    if (KT >= AHEAD)
+        landed(integral_constant<int, (AHEAD - 1) * T>{}, integral_constant<int, AHEAD - 1>{});
+    else
+        landed(none{}, none{});
     read_w(0, 0, 0);
     read_s(0);
 #pragma unroll
     for (int i = 0; i < TI; i++) read_x(i, 0);
-    uint32_t at = 0;
+    uint32_t at = 0, prev = (NB - 1) * STAGE;
     for (int st = 0; st < KT - 1; st++) {
         const uint32_t next = at == (NB - 1) * STAGE ? 0 : at + STAGE;
-        stage(std::false_type{}, st, at, next);
-        at = next;
+        stage(std::false_type{}, st, at, next, prev);
+        prev = at, at = next;
     }
-    stage(std::true_type{}, KT - 1, at, 0);
+    stage(std::true_type{}, KT - 1, at, 0, 0);
     __syncthreads();  // (nothing is under way: the last requests were waited for a stage ago)
 
     // ---- epilogue: a lane holds token 16 i + r and channels 16 j + 4 c .. + 3.  A wavefront stages 32 tokens at a time in
