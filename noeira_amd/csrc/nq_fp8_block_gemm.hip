@@ -72,12 +72,18 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     const float* const sbase = sx_wave ? p.xs + (int64_t)m0 * p.G : p.ws + (int64_t)(n0 / 128) * p.G;
     const int srow_end = sx_wave ? p.M - m0 : (p.N + 127) / 128 - n0 / 128;
     const uint32_t scales0 = NB * STAGE;
-    auto scale_dma = [&](int chunk, int quarter) {
+    int iq = 0, ichunk = 4;               // what the next stage requested brings along: quarter iq of the chunk from stage ichunk on
+    uint32_t ibuf = scales0 + CHUNK_BYTES;  // ... and the buffer it goes to
+    auto scale_dma = [&](int quarter, int from, uint32_t buffer) {
         const int row = sx_wave ? (quarter * SW + wave) * 16 + lane / 4 : lane / 4;
-        const uint32_t o = ((uint32_t)min(row, srow_end - 1) * (uint32_t)p.G + (uint32_t)min(4 * chunk + lane % 4, p.G - 1)) * 4;
-        const uint32_t m0v = lds0 + scales0 + (uint32_t)(chunk % 3) * CHUNK_BYTES + (sx_wave ? (uint32_t)(quarter * SW + wave) * 256 : BM * 16);
+        const uint32_t o = ((uint32_t)min(row, srow_end - 1) * (uint32_t)p.G + (uint32_t)min(from + lane % 4, p.G - 1)) * 4;
+        const uint32_t m0v = lds0 + buffer + (sx_wave ? (uint32_t)(quarter * SW + wave) * 256 : BM * 16);
         const float* s = sbase;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
+    };
+    auto next_scales = [&]() {
+        if (scaling) scale_dma(iq, ichunk, ibuf);
+        if (++iq == 4) iq = 0, ichunk += 4, ibuf = ibuf == scales0 + 2 * CHUNK_BYTES ? scales0 : ibuf + CHUNK_BYTES;
     };
     // K ends inside the last block: pieces behind it come from the weight's own padding, which is zero there (a piece of
     // 16 behind K exists in the first tile's last block, its very last)
@@ -85,11 +91,12 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     const uint8_t* const zeros = p.w + (int64_t)(p.G - 1) * 2048 + 1024 + 48 * 16;
     const int KT = p.G;
     // transfer t of stage st into the buffer at LDS address `at`
-    auto dma = [&](auto tc, int st, uint32_t at) {
+    auto dma = [&](auto tc, auto fullc, int st, uint32_t at) {
         constexpr int t = decltype(tc)::value;
+        constexpr bool FULL = decltype(fullc)::value;  // the stage is known to be a whole block of K
         if constexpr (t < DX) {
             const uint32_t m0v = at + (uint32_t)(wave * DX + t) * 1024;
-            if (ragged && st == KT - 1) {
+            if (!FULL && ragged && st == KT - 1) {
                 const uint8_t* a = st * 128 + xk[t] < p.K ? xbase + xoff[t] + (int64_t)st * 128 : zeros;
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0v), "v"(a) : "memory");
             } else {
@@ -138,12 +145,15 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             for (int e = 0; e < 2; e++)
                 wf[set][h][e] = *reinterpret_cast<const i32x4*>(lds + at + fw + (2 * pair + h) * 2048 + e * 1024);
     };
-    auto read_s = [&](int st) {
-        const uint32_t o = (uint32_t)(st / 4 % 3) * CHUNK_BYTES + (uint32_t)(st % 4) * 4;
+    uint32_t so = 0;  // where the next stage's scales lie
+    auto read_s = [&]() {
 #pragma unroll
-        for (int i = 0; i < TI; i++) sx[i] = *reinterpret_cast<const float*>(lds + o + fs + i * 256);
-        sw = *reinterpret_cast<const float*>(lds + o + fsw);
+        for (int i = 0; i < TI; i++) sx[i] = *reinterpret_cast<const float*>(lds + so + fs + i * 256);
+        sw = *reinterpret_cast<const float*>(lds + so + fsw);
+        so += 4;
+        if ((so & 15) == 0) so = so == 2 * CHUNK_BYTES + 16 ? 0 : so + CHUNK_BYTES - 16;
     };
+    static_assert(CHUNK_BYTES % 16 == 0, "read_s counts by it");
 
     f32x4 acc[TI][TJ];
 #pragma unroll
@@ -165,9 +175,13 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     // the middle pairs, the w half by the stage's own barrier, refilled during its last pair and the next one's first.
     constexpr int Q = TI * TJ, QB = Q - 2 * TI;  // products of a stage; the first one behind its barrier
     constexpr int T = DX + DW;
-    auto stage = [&](auto lastc, int st, uint32_t at, uint32_t next, uint32_t prev) {
-        constexpr bool LAST = decltype(lastc)::value;
-        const bool more = st + (NB >= 3 ? NB - 1 : 2) < KT;
+    constexpr int AHEAD = NB >= 3 ? NB - 1 : 2;  // stages requested before the first
+    // KIND 0: what it requests exists and is a whole block of K (no branches); 1: any stage but the last; 2: the last
+    auto stage = [&](auto kindc, int st, uint32_t at, uint32_t next, uint32_t prev) {
+        constexpr int KIND = decltype(kindc)::value;
+        constexpr bool LAST = KIND == 2;
+        using full = integral_constant<bool, KIND == 0>;
+        const bool more = KIND == 0 || st + AHEAD < KT;
         float s[TI];
         f32x4 part[3];
         auto settle = [&](int q) {  // product q of the stage: pair q / (2 TI), token (q / 2) % TI, half q % 2
@@ -183,7 +197,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             constexpr int q = decltype(qc)::value;
             auto some = [&](auto firstc, auto endc, int to, uint32_t buffer) {
                 constexpr int first = decltype(firstc)::value, end = decltype(endc)::value;
-                static_for<end - first>([&](auto d) { dma(integral_constant<int, first + decltype(d)::value>{}, to, lds0 + buffer); });
+                static_for<end - first>([&](auto d) { dma(integral_constant<int, first + decltype(d)::value>{}, full{}, to, lds0 + buffer); });
             };
             if constexpr (LAST) {
             } else if constexpr (NB >= 3) {
@@ -191,19 +205,19 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 if constexpr (to > from)
                     if (more) some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + NB - 1, prev);
                 if constexpr (q == Q - 1)
-                    if (more && scaling) scale_dma((st + NB - 1) / 4 + 1, (st + NB - 1) % 4);
+                    if (more) next_scales();
             } else {
                 constexpr int HALF = DW / 2, FIRST = 2 * TI;  // products of the first pair, and of the last
                 if constexpr (q < FIRST) {
                     constexpr int from = DX + HALF + q * (DW - HALF) / FIRST, to = DX + HALF + (q + 1) * (DW - HALF) / FIRST;
                     if constexpr (to > from)
-                        if (st > 0) some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + 1, next);
+                        some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + 1, next);
                 } else if constexpr (q < QB) {
                     constexpr int from = (q - FIRST) * DX / (QB - FIRST), to = (q - FIRST + 1) * DX / (QB - FIRST);
                     if constexpr (to > from)
                         if (more) some(integral_constant<int, from>{}, integral_constant<int, to>{}, st + 2, at);
                     if constexpr (q == QB - 1)
-                        if (more && scaling) scale_dma((st + 2) / 4 + 1, (st + 2) % 4);
+                        if (more) next_scales();
                 } else {
                     constexpr int from = DX + (q - QB) * HALF / FIRST, to = DX + (q - QB + 1) * HALF / FIRST;
                     if constexpr (to > from)
@@ -243,7 +257,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                         landed(none{}, none{});
                 }
                 read_w((pr + 1) & 1, 0, next);
-                read_s(st + 1);
+                read_s();
             }
             __builtin_amdgcn_sched_barrier(0);
             const Operand<EXACT> w0(wf[pr & 1][0][0], wf[pr & 1][0][1]), w1(wf[pr & 1][1][0], wf[pr & 1][1][1]);
@@ -268,28 +282,37 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
         settle(Q - 1);
     };
 
-    constexpr int AHEAD = NB >= 3 ? NB - 1 : 2;  // stages requested before the first
     if (scaling)
-        for (int q = 0; q < 4; q++) scale_dma(0, q);
+        for (int q = 0; q < 4; q++) scale_dma(q, 0, scales0);
+    // (two buffers: the second half of stage 1's weights follows in stage 0, as in every stage)
+    constexpr int SECOND = NB >= 3 ? T : DX + DW / 2;
     for (int st = 0; st < min(AHEAD, KT); st++) {
-        static_for<T>([&](auto t) { dma(t, st, lds0 + st * STAGE); });
-        if (scaling) scale_dma(st / 4 + 1, st % 4);
+        if (NB >= 3 || st == 0)
+            static_for<T>([&](auto t) { dma(t, std::false_type{}, st, lds0 + st * STAGE); });
+        else
+            static_for<SECOND>([&](auto t) { dma(t, std::false_type{}, st, lds0 + st * STAGE); });
+        next_scales();
     }
     if (KT >= AHEAD)
-        landed(integral_constant<int, (AHEAD - 1) * T>{}, integral_constant<int, AHEAD - 1>{});
+        landed(integral_constant<int, (AHEAD - 1) * SECOND>{}, integral_constant<int, AHEAD - 1>{});
     else
         landed(none{}, none{});
     read_w(0, 0, 0);
-    read_s(0);
+    read_s();
 #pragma unroll
     for (int i = 0; i < TI; i++) read_x(i, 0);
     uint32_t at = 0, prev = (NB - 1) * STAGE;
-    for (int st = 0; st < KT - 1; st++) {
-        const uint32_t next = at == (NB - 1) * STAGE ? 0 : at + STAGE;
-        stage(std::false_type{}, st, at, next, prev);
-        prev = at, at = next;
-    }
-    stage(std::true_type{}, KT - 1, at, 0, 0);
+    int st = 0;
+    auto walk = [&](auto kindc, int end) {
+        for (; st < end; st++) {
+            const uint32_t next = at == (NB - 1) * STAGE ? 0 : at + STAGE;
+            stage(kindc, st, at, next, prev);
+            prev = at, at = next;
+        }
+    };
+    walk(integral_constant<int, 0>{}, (ragged ? KT - 1 : KT) - AHEAD);
+    walk(integral_constant<int, 1>{}, KT - 1);
+    stage(integral_constant<int, 2>{}, KT - 1, at, 0, 0);
     __syncthreads();  // (nothing is under way: the last requests were waited for a stage ago)
 
     // ---- epilogue: a lane holds token 16 i + r and channels 16 j + 4 c .. + 3.  A wavefront stages 32 tokens at a time in
