@@ -112,14 +112,11 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
         }
     };
-    // Everything this wavefront has requested has landed but for the last `keep` transfers and `scales` of scales (which
-    // only the scaling wavefronts have; transfers land in the order of issue), and so for all wavefronts behind the barrier.
-    auto landed = [&](auto keepc, auto scalesc) {
-        constexpr int keep = decltype(keepc)::value, scales = decltype(scalesc)::value;
-        if (scales > 0 && scaling)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep + scales) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(keep) : "memory");
+    // Everything this wavefront has requested has landed but for its last `keep` transfers (they land in the order of
+    // issue; the scaling wavefronts' scales are not counted, so that they wait for one transfer or two more), and so for
+    // all wavefronts behind the barrier.
+    auto landed = [&](auto keepc) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(keepc)::value) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
@@ -176,6 +173,16 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     constexpr int Q = TI * TJ, QB = Q - 2 * TI;  // products of a stage; the first one behind its barrier
     constexpr int T = DX + DW;
     constexpr int AHEAD = NB >= 3 ? NB - 1 : 2;  // stages requested before the first
+    f32x4 late[2] = {};  // the results of the stage's last two products, settled behind the next stage's first two
+    float late_s = 0.0f;
+    auto settle_into = [&](int q, const f32x4& d, float s) {
+        auto& a = acc[q / 2 % TI][2 * (q / (2 * TI)) + q % 2];
+#pragma unroll
+        for (int t = 0; t < 4; t++) a[t] = fmaf(d[t], s, a[t]);
+        // (here and not later: left alone, the compiler gathers a stage's multiply-adds behind its last product, with every
+        // product's result kept until then)
+        asm volatile("" : "+v"(a));
+    };
     // KIND 0: what it requests exists and is a whole block of K (no branches); 1: any stage but the last; 2: the last
     auto stage = [&](auto kindc, int st, uint32_t at, uint32_t next, uint32_t prev) {
         constexpr int KIND = decltype(kindc)::value;
@@ -184,14 +191,12 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
         const bool more = KIND == 0 || st + AHEAD < KT;
         float s[TI];
         f32x4 part[3];
-        auto settle = [&](int q) {  // product q of the stage: pair q / (2 TI), token (q / 2) % TI, half q % 2
-            const int i = q / 2 % TI, j = 2 * (q / (2 * TI)) + q % 2;
-#pragma unroll
-            for (int t = 0; t < 4; t++) acc[i][j][t] = fmaf(part[q % 3][t], s[i], acc[i][j][t]);
-            // (here and not later: left alone, the compiler gathers the stage's multiply-adds behind its last product, with
-            // every product's result kept until then)
-            auto& a = acc;
-            asm volatile("" : "+v"(a[i][j]));
+        auto settle = [&](auto qc) {  // product q of the stage: pair q / (2 TI), token (q / 2) % TI, half q % 2
+            constexpr int q = decltype(qc)::value;
+            if constexpr (q < 0)
+                settle_into(Q + q, late[2 + q], late_s);
+            else
+                settle_into(q, part[q % 3], s[q / 2 % TI]);
         };
         auto transfers = [&](auto qc) {  // behind product q
             constexpr int q = decltype(qc)::value;
@@ -245,16 +250,16 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 // under way may be: what this stage has requested so far, and (four buffers) the stage after the next one
                 if constexpr (NB >= 3) {
                     if (more)
-                        landed(integral_constant<int, (NB - 3) * T + QB * T / Q>{}, integral_constant<int, NB - 3>{});
+                        landed(integral_constant<int, (NB - 3) * T + QB * T / Q>{});
                     else if (NB == 4 && st + 2 < KT)
-                        landed(integral_constant<int, T>{}, integral_constant<int, 1>{});
+                        landed(integral_constant<int, T>{});
                     else
-                        landed(none{}, none{});
+                        landed(none{});
                 } else {
                     if (more)
-                        landed(integral_constant<int, DX>{}, integral_constant<int, 1>{});
+                        landed(integral_constant<int, DX>{});
                     else
-                        landed(none{}, none{});
+                        landed(none{});
                 }
                 read_w((pr + 1) & 1, 0, next);
                 read_s();
@@ -267,19 +272,18 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 const Operand<EXACT> x(xf[i][0], xf[i][1]);
                 part[q % 3] = block_sum(w0, x);
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (q >= 2) settle(q - 2);
+                settle(integral_constant<int, q - 2>{});
                 transfers(integral_constant<int, q>{});
                 __builtin_amdgcn_sched_barrier(0);
                 part[(q + 1) % 3] = block_sum(w1, x);
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (q >= 1) settle(q - 1);
+                settle(integral_constant<int, q - 1>{});
                 if constexpr (END && !LAST) read_x(i, next);
                 transfers(integral_constant<int, q + 1>{});
                 __builtin_amdgcn_sched_barrier(0);
             });
         });
-        settle(Q - 2);
-        settle(Q - 1);
+        late[0] = part[(Q - 2) % 3], late[1] = part[(Q - 1) % 3], late_s = s[TI - 1];
     };
 
     if (scaling)
@@ -294,9 +298,12 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
         next_scales();
     }
     if (KT >= AHEAD)
-        landed(integral_constant<int, (AHEAD - 1) * SECOND>{}, integral_constant<int, AHEAD - 1>{});
+        landed(integral_constant<int, (AHEAD - 1) * SECOND>{});
     else
-        landed(none{}, none{});
+        landed(none{});
+    // (a wait that the compiler sees: it would otherwise hold scalar loads of the kernel's arguments for possibly under way
+    // and, since those return in any order, wait for every LDS read at the head of each stage)
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     read_w(0, 0, 0);
     read_s();
 #pragma unroll
@@ -313,6 +320,8 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     walk(integral_constant<int, 0>{}, (ragged ? KT - 1 : KT) - AHEAD);
     walk(integral_constant<int, 1>{}, KT - 1);
     stage(integral_constant<int, 2>{}, KT - 1, at, 0, 0);
+    settle_into(Q - 2, late[0], late_s);
+    settle_into(Q - 1, late[1], late_s);
     __syncthreads();  // (nothing is under way: the last requests were waited for a stage ago)
 
     // ---- epilogue: a lane holds token 16 i + r and channels 16 j + 4 c .. + 3.  A wavefront stages 32 tokens at a time in
