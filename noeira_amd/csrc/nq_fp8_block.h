@@ -56,6 +56,7 @@ struct BlockParams {
     const void* bias;
     int32_t M, N, K, G;
     int32_t tiles_m, tiles_n;
+    int32_t m_base, n_base;  // the GEMM: its tiles count from here
     int32_t y_dtype, bias_dtype, relu;
     SegTable seg;
 };

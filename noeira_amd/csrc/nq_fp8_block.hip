@@ -270,6 +270,30 @@ int32_t launch_tile(BlockParams p, hipStream_t s) {
     return NQ_OK;
 }
 
+// The tile shapes of the few-rows kernel.  A call of it is bound by the operands' way into the CUs: a workgroup brings in
+// 16 (MT + NT) rows of K bytes at about 33 KB per microsecond and CU (8.5 TB/s over the chip, measured at M = 32 .. 512
+// over 4096 x 4096), so of the shapes the one with the lowest estimate is taken; up to two workgroups per CU the fullest CU
+// counts, beyond that the load evens out.  Measured (K = N = 4096, M = 16 / 32 / 64 / 128 / 256, us): 1 x 1 5.5 / 8.5 / 13 / - / -,
+// 1 x 2 6.0 / 7.2 / 11.7 / - / -, 2 x 2 - / 8.7 / 8.8 / 15.0 / -, 2 x 4 - / - / 11.1 / 13.3 / 22.4, 4 x 4 - / - / - / 17 / 17.4.
+struct Shape {
+    int mt, nt;
+};
+constexpr Shape SHAPES[] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}, {4, 4}};
+double tile_estimate_us(const BlockParams& p, const Shape& t) {
+    const double wgs = (double)((p.M - 1) / (16 * t.mt) + 1) * ((p.N - 1) / (16 * t.nt) + 1) / 256.0;
+    const double per_cu = wgs <= 1.0 ? 1.0 : wgs <= 2.0 ? 2.0 : wgs;
+    return 2.2 + per_cu * (double)p.K * 16.0 * (t.mt + t.nt) / 33.2e3;
+}
+const Shape* pick_shape(const BlockParams& p, double* us) {
+    const Shape* best = nullptr;
+    for (const Shape& t : SHAPES) {
+        if (16 * (t.mt - 1) >= p.M) break;  // (no tile of rows that are not there)
+        const double e = tile_estimate_us(p, t);
+        if (!best || e < *us) best = &t, *us = e;
+    }
+    return best;
+}
+
 }  // namespace
 
 int32_t launch_fp8_block_repack(const uint8_t* codes, uint8_t* tiles, int32_t rows, int32_t cols, bool transpose, hipStream_t s) {
@@ -323,21 +347,40 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
     p.M = a.M, p.N = L->out, p.K = L->in, p.G = L->groups;
     p.y_dtype = a.y_dtype, p.bias_dtype = a.bias_dtype, p.relu = a.epilogue == NQ_EPI_RELU;
     p.seg = a.seg;
+    double tile_us = 0.0;
+    const Shape* shape = pick_shape(p, &tile_us);
     if (fp8_block_gemm_applicable(p)) {
-        // the GEMM writes one part: a row-fused layer's parts one after the other (they begin on whole blocks)
+        // the GEMM writes one part: a row-fused layer's parts run one after the other (they begin on whole blocks)
+        BlockParams part[4];
+        double us = 0.0;
         for (int t = 0, r0 = 0; t < a.seg.nseg; r0 = a.seg.end[t], t++) {
-            BlockParams q = p;
+            BlockParams& q = part[t] = p;
             q.w = p.w + (int64_t)(r0 / 16) * p.G * 2048;
             q.ws = p.ws + (int64_t)(r0 / FP8_BLOCK) * p.G;
             q.bias = !p.bias ? nullptr : reinterpret_cast<const uint8_t*>(p.bias) + (int64_t)r0 * (p.bias_dtype == NQ_DT_F32 ? 4 : 2);
             q.N = a.seg.end[t] - r0;
             q.seg.nseg = 1, q.seg.end[0] = q.N, q.seg.y[0] = a.seg.y[t];
-            const int32_t rc = launch_fp8_block_gemm(q, a.stream);
-            if (rc) return rc;
+            us += fp8_block_gemm_estimate_us(q);
         }
-        return NQ_OK;
+        if (us < tile_us) {
+            for (int t = 0; t < a.seg.nseg; t++) {
+                const int32_t rc = launch_fp8_block_gemm(part[t], a.stream);
+                if (rc) return rc;
+            }
+            return NQ_OK;
+        }
     }
-    return launch_tile<1, 1, 4, 4>(p, a.stream);
+    switch (shape->mt * 8 + shape->nt) {
+        case 1 * 8 + 1:
+            // K over 16 wavefronts where each keeps two blocks and more: one row's call is bound by the loads under way
+            // (1 row, 4096 -> 11008: 9.1 us against 9.4 - 10 on 8; 11008 -> 4096: 9.0 against 10.1; 16 rows, 4096 -> 4096: 5.7 against 5.4)
+            if (p.G >= 64 || (p.M == 1 && p.G >= 32)) return launch_tile<1, 1, 16, 2>(p, a.stream);
+            return launch_tile<1, 1, 8, 2>(p, a.stream);
+        case 1 * 8 + 2: return launch_tile<1, 2, 8, 2>(p, a.stream);
+        case 2 * 8 + 2: return launch_tile<2, 2, 8, 2>(p, a.stream);
+        case 2 * 8 + 4: return launch_tile<2, 4, 4, 1>(p, a.stream);
+        default: return launch_tile<4, 4, 4, 1>(p, a.stream);
+    }
 }
 
 }  // namespace nq

@@ -45,7 +45,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     constexpr int GM = 8;
     const int band = lid / (GM * p.tiles_n), in_band = lid - band * GM * p.tiles_n;
     const int band_rows = min(GM, p.tiles_m - band * GM);
-    const int m0 = (band * GM + in_band % band_rows) * BM, n0 = in_band / band_rows * BN;
+    const int m0 = p.m_base + (band * GM + in_band % band_rows) * BM, n0 = p.n_base + in_band / band_rows * BN;
 
     // ---- transfers.  x: 8 rows of 128 B per instruction, the 16-byte slots of a row permuted on the way (swz) so that the
     // fragment reads below meet no bank twice; w: 1 KiB of operand order as it lies; scales: one float per lane.
@@ -392,23 +392,71 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
 template <int BM, int BN, int NB>
 constexpr size_t lds_bytes() { return (size_t)NB * (BM + BN) * 128 + 3 * (BM * 16 + 256); }
 
-// eight wavefronts, 4 x 2, two per SIMD
-template <int BM, int BN, int NB, bool EXACT>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_block_gemm_kernel(const BlockParams p) {
-    block_gemm_body<BM, BN, 4, 2, NB, EXACT>(p);
+template <int BM, int BN, int WM, int WN, int NB, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_block_gemm_kernel(const BlockParams p) {
+    block_gemm_body<BM, BN, WM, WN, NB, EXACT>(p);
 }
 
-template <int BM, int BN, int NB, bool EXACT>
-int32_t launch(BlockParams p, hipStream_t s) {
+// `grid`: the first that many tiles of the order only (0: all of the region from m_base, n_base on)
+template <int BM, int BN, int WM, int WN, int NB, bool EXACT>
+int32_t launch(BlockParams p, hipStream_t s, int64_t grid = 0) {
     static LdsAttrOnce attr;
-    p.tiles_m = (p.M - 1) / BM + 1, p.tiles_n = (p.N - 1) / BN + 1;
-    const int64_t grid = (int64_t)p.tiles_m * p.tiles_n;
+    p.tiles_m = (p.M - p.m_base - 1) / BM + 1, p.tiles_n = (p.N - p.n_base - 1) / BN + 1;
+    if (grid == 0) grid = (int64_t)p.tiles_m * p.tiles_n;
     if (grid * 512 > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
-    const void* kernel = reinterpret_cast<const void*>(&fp8_block_gemm_kernel<BM, BN, NB, EXACT>);
+    const void* kernel = reinterpret_cast<const void*>(&fp8_block_gemm_kernel<BM, BN, WM, WN, NB, EXACT>);
     NQ_HIP(set_max_lds_once(attr, kernel, lds_bytes<BM, BN, NB>()));
-    hipLaunchKernelGGL((fp8_block_gemm_kernel<BM, BN, NB, EXACT>), dim3((unsigned)grid), dim3(512), (lds_bytes<BM, BN, NB>()), s, p);
+    hipLaunchKernelGGL((fp8_block_gemm_kernel<BM, BN, WM, WN, NB, EXACT>), dim3((unsigned)grid), dim3(64 * WM * WN), (lds_bytes<BM, BN, NB>()), s, p);
     NQ_HIP(hipGetLastError());
     return NQ_OK;
+}
+
+// What a call takes on each tile, in microseconds: rounds of as many workgroups as the chip holds, each a fixed part and a
+// part per block of K, which lengthens as more CUs draw on L2 (`crowd`: from 0 at `from` workgroups to 1 at `full`).
+// Measured over M = 256 .. 8192, K = 960 and 4096, N = 960 .. 11008 (K = 4096, N = 4096; M = 256 / 512 / 1024 / 2048 / 4096):
+//   bf16 y   128 x 128: 18.2 / 18.5 / 20.6 / 44.6 / 89     128 x 256: 26.7 / 27.0 / 27.7 / 35.8 / 71
+//            256 x 256: 46.5 / 46.8 / 47.1 / 50.1 / 60.4
+//   fp32 y    64 x 128: 26.0 / 26.6 / 39.6 / 77 / 153      128 x 128: 33.7 / 34.5 / 36.8 / 72 / 141
+//            256 x 128: 54.1 / 54.8 / 56.6 / 61.5 / 120
+struct Form {
+    int bm, bn;
+    double fixed, step, crowd;
+    int from, full;
+};
+constexpr Form F256{256, 256, 8.0, 1.20, 0.40, 64, 256}, F128x256{128, 256, 5.8, 0.665, 0.275, 128, 256},
+    F128{128, 128, 4.5, 0.44, 0.06, 128, 256}, E256x128{256, 128, 6.5, 1.52, 0.20, 64, 256},
+    E128{128, 128, 4.5, 0.92, 0.09, 128, 256}, E64{64, 128, 4.5, 0.69, 0.41, 256, 512};
+
+double estimate(const Form& f, int64_t workgroups, int G) {
+    const int64_t rounds = (workgroups + f.full - 1) / f.full;
+    const double in_round = (double)workgroups / (double)rounds;
+    const double crowd = in_round > f.from ? (in_round - f.from) / (double)(f.full - f.from) : 0.0;
+    return (double)rounds * (f.fixed + G * (f.step + f.crowd * crowd));
+}
+double estimate(const Form& f, int M, int N, int G) { return estimate(f, (int64_t)((M - 1) / f.bm + 1) * ((N - 1) / f.bn + 1), G); }
+
+// The 256 x 256 tiles that do not fill a round of 256 workgroups go on 128 x 256 tiles in a second launch, where they are
+// at most half a round and whole columns of the last band of 8 row tiles (M = 8192, N = 11008: 96 of 1376, 12 columns).
+// Every result adds the same blocks in the same order on any tile: same bits.
+int64_t leftover(int M, int N) {
+    const int64_t tm = (M - 1) / 256 + 1, tn = (N - 1) / 256 + 1, rest = tm * tn % 256, rows = tm - (tm - 1) / 8 * 8;
+    return tm * tn > 256 && rest > 0 && rest <= 128 && rest % rows == 0 && rest / rows <= tn ? rest : 0;
+}
+double estimate256(int M, int N, int G) {
+    const int64_t tiles = (int64_t)((M - 1) / 256 + 1) * ((N - 1) / 256 + 1), rest = leftover(M, N);
+    return rest ? estimate(F256, tiles - rest, G) + estimate(F128x256, 2 * rest, G) : estimate(F256, tiles, G);
+}
+
+// the form of lowest estimate and that estimate
+const Form* pick(const BlockParams& p, double* us) {
+    const bool exact = p.y_dtype == NQ_DT_F32;
+    const Form* best = exact ? &E256x128 : &F256;
+    *us = exact ? estimate(E256x128, p.M, p.N, p.G) : estimate256(p.M, p.N, p.G);
+    for (const Form* f : {exact ? &E128 : &F128x256, exact ? &E64 : &F128}) {
+        const double t = estimate(*f, p.M, p.N, p.G);
+        if (t < *us) *us = t, best = f;
+    }
+    return best;
 }
 
 }  // namespace
@@ -418,12 +466,28 @@ bool fp8_block_gemm_applicable(const BlockParams& p) {
     return p.M > 64 && (int64_t)p.K * 256 < ((int64_t)1 << 32);
 }
 
-double fp8_block_gemm_estimate_us(const BlockParams& p) { return p.M > 64 ? 0.0 : 1e9; }
+double fp8_block_gemm_estimate_us(const BlockParams& p) {
+    double us;
+    pick(p, &us);
+    return us;
+}
 
 int32_t launch_fp8_block_gemm(const BlockParams& p, hipStream_t s) {
-    if (p.y_dtype == NQ_DT_F32) return launch<128, 128, 4, true>(p, s);
-    if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) < 128) return launch<128, 128, 4, false>(p, s);
-    return launch<256, 256, 2, false>(p, s);
+    double us;
+    const Form* f = pick(p, &us);
+    if (f == &E64) return launch<64, 128, 2, 2, 3, true>(p, s);
+    if (f == &E128) return launch<128, 128, 4, 2, 4, true>(p, s);
+    if (f == &E256x128) return launch<256, 128, 4, 2, 3, true>(p, s);
+    if (f == &F128) return launch<128, 128, 4, 2, 4, false>(p, s);
+    if (f == &F128x256) return launch<128, 256, 4, 2, 3, false>(p, s);
+    const int64_t rest = leftover(p.M, p.N);
+    if (!rest) return launch<256, 256, 4, 2, 2, false>(p, s);
+    const int tm = (p.M - 1) / 256 + 1, tn = (p.N - 1) / 256 + 1, rows = tm - (tm - 1) / 8 * 8;
+    const int32_t rc = launch<256, 256, 4, 2, 2, false>(p, s, (int64_t)tm * tn - rest);
+    if (rc) return rc;
+    BlockParams q = p;
+    q.m_base = (tm - rows) * 256, q.n_base = (tn - (int)(rest / rows)) * 256;
+    return launch<128, 256, 4, 2, 3, false>(q, s);
 }
 
 }  // namespace nq
