@@ -58,6 +58,7 @@ struct BlockParams {
     int32_t tiles_m, tiles_n;
     int32_t m_base, n_base;  // the GEMM: its tiles count from here
     int32_t y_dtype, bias_dtype, relu;
+    int32_t vec;  // the few-rows kernel: y can be written four channels at a time
     SegTable seg;
 };
 

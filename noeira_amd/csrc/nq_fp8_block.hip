@@ -25,6 +25,8 @@
 #include "nq_fp8_block.h"
 #include "nq_fp8_quant.h"
 
+#include <type_traits>
+
 namespace nq {
 
 namespace {
@@ -210,49 +212,42 @@ __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockPara
 #pragma unroll
         for (int j = 0; j < NT; j++) *reinterpret_cast<f32x4*>(&part[wave][16 * i + r][16 * j + 4 * c]) = acc[i][j];
     __syncthreads();
-    // four channels of a row per thread, a part's boundary never among them (parts begin on a multiple of 128)
-    for (int o = threadIdx.x; o < ROWS * CH / 4; o += 64 * KW) {
-        const int row = o / (CH / 4), ch = o % (CH / 4) * 4;
-        const int m = m0 + row, n = n0 + ch;
-        if (m >= p.M || n >= p.N) continue;
-        f32x4 z = *reinterpret_cast<const f32x4*>(&part[0][row][ch]);
+    auto finish = [&](float z, int n) {
+        if (p.bias)
+            z += p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[n]
+                                           : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[n] << 16);
+        return p.relu ? (z > 0.0f ? z : 0.0f) : z;
+    };
+    typedef typename std::conditional<EXACT, float, __bf16>::type out_t;
+    void* y;
+    int width, col;
+    if (p.vec) {  // four channels of a row per thread (OUT % 4 == 0: a part's boundary or end never among them)
+        for (int o = threadIdx.x; o < ROWS * CH / 4; o += 64 * KW) {
+            const int row = o / (CH / 4), ch = o % (CH / 4) * 4;
+            const int m = m0 + row, n = n0 + ch;
+            if (m >= p.M || n >= p.N) continue;
+            f32x4 z = *reinterpret_cast<const f32x4*>(&part[0][row][ch]);
 #pragma unroll
-        for (int w = 1; w < KW; w++) z += *reinterpret_cast<const f32x4*>(&part[w][row][ch]);
-        if (p.bias) {
+            for (int w = 1; w < KW; w++) z += *reinterpret_cast<const f32x4*>(&part[w][row][ch]);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const int nn = min(n + t, p.N - 1);
-                z[t] += p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[nn]
-                                                  : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[nn] << 16);
-            }
-        }
-        if (p.relu) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) z[t] = z[t] > 0.0f ? z[t] : 0.0f;
-        }
-        void* y;
-        int width, col;
-        seg_lookup(p.seg, n, y, width, col);
-        const int64_t at = (int64_t)m * width + col;
-        if (EXACT) {
-            float* q = reinterpret_cast<float*>(y) + at;
-            if (((uintptr_t)q & 15) == 0 && n + 4 <= p.N) {
+            for (int t = 0; t < 4; t++) z[t] = finish(z[t], n + t);
+            seg_lookup(p.seg, n, y, width, col);
+            out_t* q = reinterpret_cast<out_t*>(y) + (int64_t)m * width + col;
+            if constexpr (EXACT)
                 *reinterpret_cast<f32x4*>(q) = z;
-            } else {
+            else
+                *reinterpret_cast<bf16x4*>(q) = __builtin_convertvector(z, bf16x4);
+        }
+    } else {  // one channel per thread, adjacent threads adjacent
+        for (int o = threadIdx.x; o < ROWS * CH; o += 64 * KW) {
+            const int row = o / CH, ch = o % CH;
+            const int m = m0 + row, n = n0 + ch;
+            if (m >= p.M || n >= p.N) continue;
+            float z = part[0][row][ch];
 #pragma unroll
-                for (int t = 0; t < 4; t++)
-                    if (n + t < p.N) q[t] = z[t];
-            }
-        } else {
-            const bf16x4 b = __builtin_convertvector(z, bf16x4);
-            __bf16* q = reinterpret_cast<__bf16*>(y) + at;
-            if (((uintptr_t)q & 7) == 0 && n + 4 <= p.N) {
-                *reinterpret_cast<bf16x4*>(q) = b;
-            } else {
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-                    if (n + t < p.N) q[t] = b[t];
-            }
+            for (int w = 1; w < KW; w++) z += part[w][row][ch];
+            seg_lookup(p.seg, n, y, width, col);
+            reinterpret_cast<out_t*>(y)[(int64_t)m * width + col] = (out_t)finish(z, n);
         }
     }
 }
@@ -282,7 +277,9 @@ constexpr Shape SHAPES[] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}, {4, 4}};
 double tile_estimate_us(const BlockParams& p, const Shape& t) {
     const double wgs = (double)((p.M - 1) / (16 * t.mt) + 1) * ((p.N - 1) / (16 * t.nt) + 1) / 256.0;
     const double per_cu = wgs <= 1.0 ? 1.0 : wgs <= 2.0 ? 2.0 : wgs;
-    return 2.2 + per_cu * (double)p.K * 16.0 * (t.mt + t.nt) / 33.2e3;
+    // (every workgroup after a CU's first adds its meeting in LDS and its stores: 128 k over 8192 x 11008 outputs in tiles of
+    // 4 x 4 took 1.9 us a workgroup)
+    return 2.2 + per_cu * (double)p.K * 16.0 * (t.mt + t.nt) / 33.2e3 + (per_cu - 1.0) * 0.1 * t.mt * t.nt;
 }
 const Shape* pick_shape(const BlockParams& p, double* us) {
     const Shape* best = nullptr;
@@ -347,6 +344,9 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
     p.M = a.M, p.N = L->out, p.K = L->in, p.G = L->groups;
     p.y_dtype = a.y_dtype, p.bias_dtype = a.bias_dtype, p.relu = a.epilogue == NQ_EPI_RELU;
     p.seg = a.seg;
+    const uintptr_t line = a.y_dtype == NQ_DT_F32 ? 15 : 7;  // four channels of y
+    p.vec = L->out % 4 == 0;
+    for (int t = 0; t < a.seg.nseg; t++) p.vec = p.vec && ((uintptr_t)a.seg.y[t] & line) == 0;
     double tile_us = 0.0;
     const Shape* shape = pick_shape(p, &tile_us);
     if (fp8_block_gemm_applicable(p)) {
@@ -378,7 +378,11 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
             return launch_tile<1, 1, 8, 2>(p, a.stream);
         case 1 * 8 + 2: return launch_tile<1, 2, 8, 2>(p, a.stream);
         case 2 * 8 + 2: return launch_tile<2, 2, 8, 2>(p, a.stream);
-        case 2 * 8 + 4: return launch_tile<2, 4, 4, 1>(p, a.stream);
+        case 2 * 8 + 4:
+            // (a few blocks of K: one per wavefront.  135 rows, 960 -> 2567: 5.9 / 6.5 us against 6.7 / 7.1; 128 rows, 4096 -> 4096 in
+            // fp32: 16.7 against 13.5)
+            if (p.G <= 16) return launch_tile<2, 4, 8, 1>(p, a.stream);
+            return launch_tile<2, 4, 4, 1>(p, a.stream);
         default: return launch_tile<4, 4, 4, 1>(p, a.stream);
     }
 }

@@ -363,23 +363,37 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        constexpr int LPR = CH * ES / 16, RPI = 64 / LPR;  // lanes per row, rows per instruction
+        if (whole) {
+            constexpr int LPR = CH * ES / 16, RPI = 64 / LPR;  // lanes per row, rows per instruction
 #pragma unroll
-        for (int t = 0; t < 32 / RPI; t++) {
-            const int row = t * RPI + lane / LPR, c16 = lane % LPR;
-            const i32x4 v = *reinterpret_cast<const i32x4*>(stg + row * ROWB + c16 * 16);
-            const int m = wm0 + 16 * ip + row, n = wn0 + c16 * (16 / ES);
-            if (m >= p.M) continue;
-            if (whole) {
-                *reinterpret_cast<i32x4*>(y + ((int64_t)m * p.N + n) * ES) = v;
-            } else {
+            for (int t = 0; t < 32 / RPI; t++) {
+                const int row = t * RPI + lane / LPR, c16 = lane % LPR;
+                const i32x4 v = *reinterpret_cast<const i32x4*>(stg + row * ROWB + c16 * 16);
+                const int m = wm0 + 16 * ip + row, n = wn0 + c16 * (16 / ES);
+                if (m < p.M) *reinterpret_cast<i32x4*>(y + ((int64_t)m * p.N + n) * ES) = v;
+            }
+        } else {
+            // rows that do not begin on 16 bytes, or end inside the tile: a row at a time, 4 bytes per lane, adjacent lanes
+            // adjacent (bf16 rows that begin on an odd element: pairs from the second one on, and the ends alone)
+            const int limit = min(CH, p.N - wn0);
+#pragma unroll 4
+            for (int row = 0; row < 32; row++) {
+                const int m = wm0 + 16 * ip + row;
+                if (m >= p.M) break;
+                const int64_t first = (int64_t)m * p.N + wn0;
+                const uint8_t* src = stg + row * ROWB;
+                if constexpr (EXACT) {
 #pragma unroll
-                for (int e = 0; e < 16 / ES; e++) {
-                    if (n + e >= p.N) break;
-                    if constexpr (EXACT)
-                        reinterpret_cast<int32_t*>(y)[(int64_t)m * p.N + n + e] = v[e];
-                    else
-                        reinterpret_cast<uint16_t*>(y)[(int64_t)m * p.N + n + e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+                    for (int e = lane; e < CH; e += 64)
+                        if (e < limit) reinterpret_cast<float*>(y)[first + e] = reinterpret_cast<const float*>(src)[e];
+                } else {
+                    const int odd = (int)(((uintptr_t)y / 2 + first) & 1);
+                    const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+                    uint16_t* d16 = reinterpret_cast<uint16_t*>(y) + first;
+                    for (int e = odd + 2 * lane; e + 1 < limit; e += 128)
+                        *reinterpret_cast<uint32_t*>(d16 + e) = (uint32_t)s16[e] | (uint32_t)s16[e + 1] << 16;
+                    if (lane == 0 && odd && limit > 0) d16[0] = s16[0];
+                    if (lane == 1 && limit > odd && ((limit - odd) & 1)) d16[limit - 1] = s16[limit - 1];
                 }
             }
         }
