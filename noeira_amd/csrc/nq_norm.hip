@@ -26,35 +26,28 @@ namespace {
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 
 __device__ __forceinline__ float load1(const void* p, int32_t dtype, int64_t i) {
     return dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p)[i]
                               : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
 }
 
-__device__ __forceinline__ uint32_t bf16_bits(float v) {
-    const uint32_t b = __float_as_uint(v);
-    return (b & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC0u : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
-}
-
 __device__ __forceinline__ void store1(void* p, int32_t dtype, int64_t i, float v) {
     if (dtype == NQ_DT_F32)
         reinterpret_cast<float*>(p)[i] = v;
     else
-        reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)bf16_bits(v);
+        reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
-}
 // sum over a wavefront, the same bits in every lane: neighbours, pairs, halves and rows of 16 by exchanges in which both
 // sides add the same two numbers, then the four rows
 __device__ __forceinline__ float wave_sum(float v) {
-    v += dpp<0xB1>(v);   // lane ^ 1
-    v += dpp<0x4E>(v);   // lane ^ 2
-    v += dpp<0x141>(v);  // the other quad of 8
-    v += dpp<0x140>(v);  // the other half of 16
+    v += lane_move<0xB1>(v);   // lane ^ 1
+    v += lane_move<0x4E>(v);   // lane ^ 2
+    v += lane_move<0x141>(v);  // the other quad of 8
+    v += lane_move<0x140>(v);  // the other half of 16
     const int i = __float_as_int(v);
     return (__int_as_float(__builtin_amdgcn_readlane(i, 0)) + __int_as_float(__builtin_amdgcn_readlane(i, 16))) +
            (__int_as_float(__builtin_amdgcn_readlane(i, 32)) + __int_as_float(__builtin_amdgcn_readlane(i, 48)));
@@ -124,10 +117,8 @@ __device__ __forceinline__ void put(void* out, int32_t dtype, int64_t base, int 
             f32x4* p = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(out) + base + k);
             p[0] = f32x4{f[0], f[1], f[2], f[3]}, p[1] = f32x4{f[4], f[5], f[6], f[7]};
         } else {
-            u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = bf16_bits(f[2 * i]) | bf16_bits(f[2 * i + 1]) << 16;
-            *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(out) + base + k) = w;
+            *reinterpret_cast<bf16x8*>(reinterpret_cast<uint16_t*>(out) + base + k) =
+                __builtin_convertvector((f32x8{f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]}), bf16x8);
         }
     } else {
 #pragma unroll
@@ -162,8 +153,10 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const Nor
     for (int v = 0; v < NV; v++) {
         const int k = first_index<T, VEC>(t, v);
         Raw<false> r;
+        // (a thread's values behind the row get zeros here, so that they come out as zeros: what the last block's largest
+        // magnitude may not see)
 #pragma unroll
-        for (int i = 0; i < 8; i++) g[v][i] = 1.0f, b[v][i] = 0.0f;
+        for (int i = 0; i < 8; i++) g[v][i] = (VEC ? k : k + 16 * i) < a.D ? 1.0f : 0.0f, b[v][i] = 0.0f;
         if (a.gamma) fetch<false, VEC>(r, a.gamma, k, a.D), widen<false>(r, g[v]);
         if (a.beta) fetch<false, VEC>(r, a.beta, k, a.D), widen<false>(r, b[v]);
     }
@@ -186,12 +179,16 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const Nor
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int k = first_index<T, VEC>(t, v);
+            float part = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 f[v][i] -= mean;
-                const bool in = VEC ? k < a.D : k + 16 * i < a.D;
-                sq += in ? f[v][i] * f[v][i] : 0.0f;
+                if constexpr (VEC)
+                    part = fmaf(f[v][i], f[v][i], part);
+                else
+                    part += k + 16 * i < a.D ? f[v][i] * f[v][i] : 0.0f;
             }
+            sq += !VEC || k < a.D ? part : 0.0f;
         }
         const float rstd = 1.0f / sqrtf(team_sum<T>(sq, lds[1], wave) / d + a.eps);
         if (a.mean && t == 0) a.mean[m] = mean, a.rstd[m] = rstd;
@@ -203,10 +200,6 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const Nor
             if (a.y) {
                 put<VEC>(a.y, a.y_dtype, m * a.D, k, a.D, f[v]);
             } else {
-                // (what lies behind the row counts as zero in the last block)
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (VEC ? k >= a.D : k + 16 * i >= a.D) f[v][i] = 0.0f;
                 float s;
                 const uint2 q = quantize_block16(f[v], s);
                 if constexpr (VEC) {

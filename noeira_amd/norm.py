@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from .qlinear import _TORCH_DT, _check_dev, _dev_ptr, _need_gpu, _stream_ptr
+from .qlinear import _FLOATS, _TORCH_DT, _check_dev, _dev_ptr, _need_gpu, _stream_ptr
 
 
 class LayerNorm:
@@ -44,11 +44,15 @@ class LayerNorm:
         self.beta.copy_(new[1])
 
     def _rows(self, x: torch.Tensor, what: str) -> int:
-        _check_dev(x, f"LayerNorm.{what}: x", tuple(_TORCH_DT))
+        _check_dev(x, f"LayerNorm.{what}: x", _FLOATS)
         _check_dev(self.gamma, f"LayerNorm.{what}: gamma")
         if x.numel() % self.DIM:
             raise L.NQError(L.NQ_ERR_INVALID, f"LayerNorm.{what}: x has {x.numel()} values, not a multiple of DIM = {self.DIM}")
         return x.numel() // self.DIM
+
+    def _like(self, x: torch.Tensor, M: int, dtype: torch.dtype) -> torch.Tensor:
+        t = torch.empty_like(x, dtype=dtype)
+        return t if x.dim() == 2 and x.shape[1] == self.DIM else t.view(M, self.DIM)
 
     def _forward(self, x, out, out_dtype, stats, what):
         M = self._rows(x, what)
@@ -59,7 +63,7 @@ class LayerNorm:
         if out_dtype not in _TORCH_DT:
             raise L.NQError(L.NQ_ERR_INVALID, f"LayerNorm.{what}: y must be fp32 or bf16")
         if out is None:
-            out = torch.empty((M, self.DIM), dtype=out_dtype, device=x.device)
+            out = self._like(x, M, out_dtype)
         mean = torch.empty((M,), dtype=torch.float32, device=x.device) if stats else None
         rstd = torch.empty_like(mean) if stats else None
         L.check(L.lib().nq_layer_norm(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(self.gamma), _dev_ptr(self.beta),
@@ -77,7 +81,7 @@ class LayerNorm:
 
     def _forward_fp8(self, x, stats, what):
         M = self._rows(x, what)
-        codes = torch.empty((M, self.DIM), dtype=torch.float8_e4m3fn, device=x.device)
+        codes = self._like(x, M, torch.float8_e4m3fn)
         scales = torch.empty((M, -(-self.DIM // 128)), dtype=torch.float32, device=x.device)
         mean = torch.empty((M,), dtype=torch.float32, device=x.device) if stats else None
         rstd = torch.empty_like(mean) if stats else None
@@ -99,13 +103,13 @@ class LayerNorm:
         """(grad_input [M, DIM] of x's type, dgamma, dbeta fp32 [DIM]) from the forward's input and statistics;
         ``params=False`` (a frozen norm): no sums over the rows, dgamma and dbeta are None."""
         M = self._rows(x, "vjp")
-        _check_dev(grad_output, "LayerNorm.vjp: grad_output", tuple(_TORCH_DT), M * self.DIM)
+        _check_dev(grad_output, "LayerNorm.vjp: grad_output", _FLOATS, M * self.DIM)
         _check_dev(mean, "LayerNorm.vjp: mean", torch.float32, M)
         _check_dev(rstd, "LayerNorm.vjp: rstd", torch.float32, M)
         if grad_input is None:
-            grad_input = torch.empty((M, self.DIM), dtype=x.dtype, device=x.device)
+            grad_input = self._like(x, M, x.dtype)
         else:
-            _check_dev(grad_input, "LayerNorm.vjp: grad_input", tuple(_TORCH_DT), M * self.DIM)
+            _check_dev(grad_input, "LayerNorm.vjp: grad_input", _FLOATS, M * self.DIM)
         dg = db = ws = None
         n = 0
         if params:

@@ -28,6 +28,7 @@ Q4_GROUP = 32
 Q4_BLOCK = 18
 
 _TORCH_DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}
+_FLOATS = tuple(_TORCH_DT)
 
 
 # (the stream's address without a Stream object around it: 0.3 us a call instead of 2.8)
@@ -38,6 +39,10 @@ def _stream_ptr() -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(torch.cuda.current_device())
+
+
+# (for tensors that are on a device already, so that the runtime is up: without the look at that)
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _need_gpu(target: str):
@@ -54,7 +59,8 @@ def _dev_ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _check_dev(t: torch.Tensor, what: str, dtype=None, numel=None):
     """A contiguous tensor on the current device (the stream the call goes to is that device's), of this type and size."""
-    if t.get_device() < 0 or t.get_device() != torch.cuda.current_device() or not t.is_contiguous():
+    at = t.get_device()
+    if at < 0 or at != _device_now() or not t.is_contiguous():
         raise L.NQError(L.NQ_ERR_INVALID, what + " must be a contiguous tensor on the current device")
     if dtype is not None and t.dtype is not dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
         raise L.NQError(L.NQ_ERR_INVALID, what + " must be " + " or ".join(str(d) for d in (dtype if isinstance(dtype, tuple) else (dtype,))))
@@ -444,8 +450,10 @@ class FP8BlockLinear(_Layer):
     @staticmethod
     def _codes(codes: torch.Tensor, scales: torch.Tensor, K: int, what: str) -> int:
         """Checks quantised rows [M, K] and their scales [M, ceil(K/128)]; returns M."""
-        _check_dev(codes, what + ": the codes", (torch.uint8, torch.float8_e4m3fn))
-        M = _check_x(codes, K, what)
+        _check_dev(codes, what + ": the codes", (torch.float8_e4m3fn, torch.uint8))
+        M = codes.numel() // K
+        if M * K != codes.numel():
+            raise L.NQError(L.NQ_ERR_INVALID, f"{what}: the codes are {codes.numel()} values, not a multiple of {K}")
         _check_dev(scales, what + ": the scales", torch.float32, M * (-(-K // 128)))
         return M
 
@@ -454,11 +462,22 @@ class FP8BlockLinear(_Layer):
         M = self._codes(x_codes, x_scales, self.IN, "FP8BlockLinear.forward_a8")
         if out_dtype not in _TORCH_DT:
             raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.forward_a8: y must be fp32 or bf16")
+        if epilogue not in ("none", "relu"):
+            raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.forward_a8: the epilogue is \"none\" or \"relu\"")
+        if bias is None:
+            bias = self.bias
+        b_dt = L.DT_F32
         if bias is not None:
-            _check_dev(bias, "FP8BlockLinear.forward_a8: bias")
-        if out is not None:
+            _check_dev(bias, "FP8BlockLinear.forward_a8: bias", _FLOATS, self.OUT)
+            b_dt = _TORCH_DT[bias.dtype]
+        if out is None:
+            out = x_codes.new_empty((M, self.OUT), dtype=out_dtype)
+        else:
             _check_dev(out, "FP8BlockLinear.forward_a8: out", out_dtype, M * self.OUT)
-        return self._forward(x_codes, L.DT_FP8_E4M3, x_scales, out, out_dtype, bias, epilogue, "FP8BlockLinear.forward_a8")
+        L.check(L.lib().nq_forward(self._h, x_codes.data_ptr(), L.DT_FP8_E4M3, x_scales.data_ptr(), out.data_ptr(),
+                                   _TORCH_DT[out_dtype], M, _dev_ptr(bias), b_dt, L.EPI_RELU if epilogue == "relu" else L.EPI_NONE,
+                                   _stream_ptr()))
+        return out
 
     def forward(self, x: torch.Tensor, bias=None, epilogue="none", out=None, out_dtype=torch.bfloat16):
         """fp32 or bf16 activations: quantised per row and block of 128, then the product (two launches)."""
@@ -475,7 +494,7 @@ class FP8BlockLinear(_Layer):
         if out_dtype not in _TORCH_DT:
             raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.vjp_a8: gx must be fp32 or bf16")
         if grad_input is None:
-            grad_input = torch.empty((M, self.IN), dtype=out_dtype, device=gy_codes.device)
+            grad_input = gy_codes.new_empty((M, self.IN), dtype=out_dtype)
         else:
             _check_dev(grad_input, "FP8BlockLinear.vjp_a8: grad_input", out_dtype, M * self.IN)
         L.check(L.lib().nq_grad_input_fp8_block(self._h, _dev_ptr(gy_codes), _dev_ptr(gy_scales), _dev_ptr(grad_input),
@@ -690,11 +709,11 @@ def quantize_rows_fp8_block(x: torch.Tensor, codes: Optional[torch.Tensor] = Non
     M, K = x.shape
     G = -(-K // 128)
     if codes is None:
-        codes = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
+        codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     else:
         _check_dev(codes, "quantize_rows_fp8_block: codes", (torch.uint8, torch.float8_e4m3fn), M * K)
     if scales is None:
-        scales = torch.empty((M, G), dtype=torch.float32, device=x.device)
+        scales = x.new_empty((M, G), dtype=torch.float32)
     else:
         _check_dev(scales, "quantize_rows_fp8_block: scales", torch.float32, M * G)
     L.check(L.lib().nq_quantize_rows_fp8_block(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(codes), _dev_ptr(scales), M, K,

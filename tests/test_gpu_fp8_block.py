@@ -68,6 +68,23 @@ def test_quantize_ties_go_to_even_and_quotients_are_ieee():
         assert np.array_equal(codes.view(torch.uint8).cpu().numpy(), want_q)
 
 
+def test_quantize_against_device_divisions():
+    """Half a million blocks against the device's own divisions and casts: every scale's significand a random one, among
+    them all ones (the largest magnitudes 448 (2 - 2^-23) 2^e)."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(16384, 4096, generator=gen, device="cuda") * torch.exp2(torch.randint(-40, 40, (16384, 1), generator=gen, device="cuda").float())
+    ones = 448 * (2 - 2.0 ** -23)  # 27 significant bits: the nearest fp32 values on both sides have quotients around it
+    x[:64, 0] = torch.tensor([np.nextafter(np.float32(ones), np.float32(s)) for s in (0, 1e9)] * 32, device="cuda") * 8
+    x[:64, 1:128].clamp_(-3000, 3000)
+    t = x.view(16384, 32, 128)
+    top = t.abs().amax(2)
+    s = top / torch.full_like(top, 448)
+    want = (t / s[:, :, None]).to(torch.float8_e4m3fn)
+    codes, scales = quantize_rows_fp8_block(x)
+    assert torch.equal(scales, s)
+    assert torch.equal(codes.view(torch.uint8), want.view(16384, 4096).view(torch.uint8))
+
+
 def test_quantize_extremes():
     tiny, huge, inf, nan = 2.0 ** -149, 3.4028235e38, np.inf, np.nan
     x = np.zeros((9, 384), np.float32)
@@ -190,6 +207,12 @@ def test_nothing_and_refusals():
         lin.forward_a8(xq, xs.t())
     with pytest.raises(NQError, match="expected 192"):
         lin.forward_a8(xq, xs, out=torch.empty((3, 48), dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(NQError, match="epilogue"):
+        lin.forward_a8(xq, xs, epilogue="swiglu")
+    with pytest.raises(NQError, match="bias has 47 values"):
+        lin.forward_a8(xq, xs, bias=torch.zeros(47, device="cuda"))
+    with pytest.raises(NQError, match="not a multiple of 256"):
+        lin.forward_a8(xq.view(-1)[:1000], xs)
     with pytest.raises(NQError, match="made with|NQ_FLAG_GRAD"):
         lin.vjp_a8(*R.random_rows(gen, 4, 48))
     x = torch.randn(4, 256, device="cuda")
