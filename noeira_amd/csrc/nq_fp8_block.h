@@ -1,9 +1,20 @@
 // Shared by the block-scaled fp8 product's kernels (nq_fp8_block.hip: few rows; nq_fp8_block_gemm.hip: many).
 #pragma once
 
+#include <type_traits>
+
 #include "nq_common.h"
 
 namespace nq {
+
+// f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<N, I + 1>(static_cast<F&&>(f));
+    }
+}
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -19,11 +30,13 @@ struct Operand;
 template <>
 struct Operand<false> {
     i32x8 v;
+    __device__ Operand() {}
     __device__ __forceinline__ Operand(const i32x4& a, const i32x4& b) : v{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]} {}
 };
 template <>
 struct Operand<true> {
     bf16x8 v[4];
+    __device__ Operand() {}
     __device__ __forceinline__ Operand(const i32x4& a, const i32x4& b) {
 #pragma unroll
         for (int s = 0; s < 4; s++)

@@ -140,7 +140,8 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void
 template <int MT, int NT, int KW, int U, bool EXACT>
 __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockParams p) {
     constexpr int ROWS = 16 * MT, CH = 16 * NT;
-    __shared__ __attribute__((aligned(16))) float part[KW][ROWS][CH + 4];
+    extern __shared__ __attribute__((aligned(16))) uint8_t meet[];
+    float(*const part)[ROWS][CH + 4] = reinterpret_cast<float(*)[ROWS][CH + 4]>(meet);  // [KW]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, c = lane >> 4;
@@ -192,13 +193,15 @@ __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockPara
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (g0 + u * KW < p.G) {
+                Operand<EXACT> w[NT];
 #pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const Operand<EXACT> w(wv[u][j][0], wv[u][j][1]);
+                for (int j = 0; j < NT; j++) w[j] = Operand<EXACT>(wv[u][j][0], wv[u][j][1]);
 #pragma unroll
-                    for (int i = 0; i < MT; i++) {
-                        const Operand<EXACT> x(xv[u][i][0], xv[u][i][1]);
-                        const f32x4 d = block_sum(w, x);
+                for (int i = 0; i < MT; i++) {
+                    const Operand<EXACT> x(xv[u][i][0], xv[u][i][1]);
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {
+                        const f32x4 d = block_sum(w[j], x);
                         const float s = sx[u][i] * sw[u][j];
 #pragma unroll
                         for (int t = 0; t < 4; t++) acc[i][j][t] = fmaf(d[t], s, acc[i][j][t]);
@@ -257,16 +260,21 @@ int32_t launch_tile(BlockParams p, hipStream_t s) {
     p.tiles_m = (p.M + 16 * MT - 1) / (16 * MT);
     const int64_t grid = (int64_t)p.tiles_m * ((p.N + 16 * NT - 1) / (16 * NT));
     if (grid > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
-    if (p.y_dtype == NQ_DT_F32)
-        hipLaunchKernelGGL((fp8_block_tile_kernel<MT, NT, KW, U, true>), dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
-    else
-        hipLaunchKernelGGL((fp8_block_tile_kernel<MT, NT, KW, U, false>), dim3((unsigned)grid), dim3(64 * KW), 0, s, p);
+    constexpr size_t lds = sizeof(float) * KW * 16 * MT * (16 * NT + 4);
+    static LdsAttrOnce attr[2];
+    if (p.y_dtype == NQ_DT_F32) {
+        if (lds > 65536) NQ_HIP(set_max_lds_once(attr[0], reinterpret_cast<const void*>(&fp8_block_tile_kernel<MT, NT, KW, U, true>), lds));
+        hipLaunchKernelGGL((fp8_block_tile_kernel<MT, NT, KW, U, true>), dim3((unsigned)grid), dim3(64 * KW), lds, s, p);
+    } else {
+        if (lds > 65536) NQ_HIP(set_max_lds_once(attr[1], reinterpret_cast<const void*>(&fp8_block_tile_kernel<MT, NT, KW, U, false>), lds));
+        hipLaunchKernelGGL((fp8_block_tile_kernel<MT, NT, KW, U, false>), dim3((unsigned)grid), dim3(64 * KW), lds, s, p);
+    }
     NQ_HIP(hipGetLastError());
     return NQ_OK;
 }
 
 // The tile shapes of the few-rows kernel.  A call of it is bound by the operands' way into the CUs: a workgroup brings in
-// 16 (MT + NT) rows of K bytes at about 33 KB per microsecond and CU (8.5 TB/s over the chip, measured at M = 32 .. 512
+// 16 (MT + NT) rows of K bytes at about 34 KB per microsecond and CU (8.7 TB/s over the chip, measured at M = 32 .. 512
 // over 4096 x 4096), so of the shapes the one with the lowest estimate is taken; up to two workgroups per CU the fullest CU
 // counts, beyond that the load evens out.  Measured (K = N = 4096, M = 16 / 32 / 64 / 128 / 256, us): 1 x 1 5.5 / 8.5 / 13 / - / -,
 // 1 x 2 6.0 / 7.2 / 11.7 / - / -, 2 x 2 - / 8.7 / 8.8 / 15.0 / -, 2 x 4 - / - / 11.1 / 13.3 / 22.4, 4 x 4 - / - / - / 17 / 17.4.
@@ -279,7 +287,7 @@ double tile_estimate_us(const BlockParams& p, const Shape& t) {
     const double per_cu = wgs <= 1.0 ? 1.0 : wgs <= 2.0 ? 2.0 : wgs;
     // (every workgroup after a CU's first adds its meeting in LDS and its stores: 128 k over 8192 x 11008 outputs in tiles of
     // 4 x 4 took 1.9 us a workgroup)
-    return 2.2 + per_cu * (double)p.K * 16.0 * (t.mt + t.nt) / 33.2e3 + (per_cu - 1.0) * 0.1 * t.mt * t.nt;
+    return 2.2 + 0.06 * t.mt * t.nt + per_cu * (double)p.K * 16.0 * (t.mt + t.nt) / 34e3 + (per_cu - 1.0) * 0.1 * t.mt * t.nt;
 }
 const Shape* pick_shape(const BlockParams& p, double* us) {
     const Shape* best = nullptr;
@@ -378,12 +386,16 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
             return launch_tile<1, 1, 8, 2>(p, a.stream);
         case 1 * 8 + 2: return launch_tile<1, 2, 8, 2>(p, a.stream);
         case 2 * 8 + 2: return launch_tile<2, 2, 8, 2>(p, a.stream);
+        // (five to sixteen blocks of K: over 8 wavefronts, one or two each.  135 rows, 960 -> 2567: 5.9 / 6.4 us (bf16 / fp32 y) against
+        // 6.7 / 7.1 on 4; 128 rows, 4096 -> 4096: 13.3 / 16.7 against 13.3 / 13.5)
         case 2 * 8 + 4:
-            // (a few blocks of K: one per wavefront.  135 rows, 960 -> 2567: 5.9 / 6.5 us against 6.7 / 7.1; 128 rows, 4096 -> 4096 in
-            // fp32: 16.7 against 13.5)
-            if (p.G <= 16) return launch_tile<2, 4, 8, 1>(p, a.stream);
+            if (p.G > 4 && p.G <= 16) return launch_tile<2, 4, 8, 1>(p, a.stream);
             return launch_tile<2, 4, 4, 1>(p, a.stream);
-        default: return launch_tile<4, 4, 4, 1>(p, a.stream);
+        // (8 wavefronts fill a CU's LDS: only where no CU gets two.  256 rows, 4096 -> 4096 in fp32: 19.6 us against 22.0 on 4; 512 rows:
+        // 37.9 against 33.6)
+        default:
+            if (p.G > 4 && (int64_t)((p.M - 1) / 64 + 1) * ((p.N - 1) / 64 + 1) <= 256) return launch_tile<4, 4, 8, 1>(p, a.stream);
+            return launch_tile<4, 4, 4, 1>(p, a.stream);
     }
 }
 

@@ -4,21 +4,11 @@
 // A stage of the K loop is one block of 128 k: x tile BM x 128 B, weight tile BN x 128 B and their scales, filled straight
 // from global memory (global_load_lds) into one of NB stage buffers.  A wavefront owns TI x TJ results of 16 x 16, and its
 // channels lie in one block of 128, so its weight scale is one number per stage.
-#include <type_traits>
-
 #include "nq_fp8_block.h"
 
 namespace nq {
 
 namespace {
-
-template <int N, int I = 0, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        static_for<N, I + 1>(static_cast<F&&>(f));
-    }
-}
 
 template <int BM, int BN, int WM, int WN, int NB, bool EXACT>
 __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
