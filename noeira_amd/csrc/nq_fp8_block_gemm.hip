@@ -312,6 +312,19 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     stage(integral_constant<int, 2>{}, KT - 1, at, 0, 0);
     settle_into(Q - 2, late[0], late_s);
     settle_into(Q - 1, late[1], late_s);
+    // (the bias is requested here, all of a lane's channels at once, into the registers that the fragments leave; a fragment at
+    // a time in the passes below, 1024 rows over 4096 -> 4096 took 23.5 us instead of 23.1)
+    float b[TJ][4];
+#pragma unroll
+    for (int j = 0; j < TJ; j++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int n = min(n0 + wn * 16 * TJ + 16 * j + 4 * c + t, p.N - 1);
+            b[j][t] = 0.0f;
+            if (p.bias)
+                b[j][t] = p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[n]
+                                                    : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[n] << 16);
+        }
     __syncthreads();  // (nothing is under way: the last requests were waited for a stage ago)
 
     // ---- epilogue: a lane holds token 16 i + r and channels 16 j + 4 c .. + 3.  A wavefront stages 32 tokens at a time in
@@ -326,21 +339,12 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     for (int ip = 0; ip < TI; ip += 2) {
 #pragma unroll
         for (int j = 0; j < TJ; j++) {
-            float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (p.bias) {
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int n = min(wn0 + 16 * j + 4 * c + t, p.N - 1);
-                    b[t] = p.bias_dtype == NQ_DT_F32 ? reinterpret_cast<const float*>(p.bias)[n]
-                                                     : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[n] << 16);
-                }
-            }
 #pragma unroll
             for (int ii = 0; ii < 2; ii++) {
                 f32x4 z;
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    z[t] = acc[ip + ii][j][t] + b[t];
+                    z[t] = acc[ip + ii][j][t] + b[j][t];
                     if (p.relu) z[t] = z[t] > 0.0f ? z[t] : 0.0f;
                 }
                 uint8_t* dst = stg + (16 * ii + r) * ROWB + (16 * j + 4 * c) * ES;

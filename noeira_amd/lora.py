@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from .qlinear import _TORCH_DT, _dev_ptr, _stream_ptr
+from .qlinear import _TORCH_DT, FP8BlockLinear, _dev_ptr, _stream_ptr
 
 
 class LoRAAdapter:
@@ -69,6 +69,11 @@ class LoRAAdapter:
         """``base.forward(x)`` and this adapter's share in one call (`nq_forward_lora`): one launch where the base
         call runs on the kernel that keeps its rows' activations resident, the two of `forward` + `forward_add`
         elsewhere.  B = 0 returns the bits of ``base.forward(x)``."""
+        if isinstance(base, FP8BlockLinear):  # its kernels read codes, the adapter the activations themselves: two steps
+            if out_dtype != torch.float32:
+                raise L.NQError(L.NQ_ERR_UNSUPPORTED, "LoRAAdapter.forward_with: an adapter beside an FP8BlockLinear adds into fp32")
+            y = base.forward(x, bias=bias, out=out, out_dtype=torch.float32)
+            return self.forward_add(x, y)
         if self.merged:
             return base.forward(x, bias=bias, out_dtype=out_dtype)
         if x.dtype not in _TORCH_DT or not x.is_cuda or not x.is_contiguous() or x.dim() != 2 or x.shape[1] != self.IN:
@@ -88,14 +93,22 @@ class LoRAAdapter:
 
 
 def proj_fwd(base, x: torch.Tensor, adapter: "LoRAAdapter | None" = None, hessian=None, bias: torch.Tensor | None = None,
-             out: torch.Tensor | None = None) -> torch.Tensor:
+             out: torch.Tensor | None = None, norm=None) -> torch.Tensor:
     """One projection of the decoder layer as the reference's caller runs it, `DecoderLayerWeights.proj_fwd`
     (noeira/deep_agents/smolvla/layer_weights.mojo:455-508): when calibrating, the projection's input is added to
     its Hessian first (`HessianAccumulator.add`, hessian.mojo:41-77: `hessian` is a `noeira_amd.gptq.HessianAccumulator` or
     None); then the base linear; then the adapter's share, if the projection carries an unmerged one.  x: fp32 or
-    bf16 [T, IN] on the device; returns fp32 [T, OUT]."""
+    bf16 [T, IN] on the device; returns fp32 [T, OUT].  `norm`: a `LayerNorm` ahead of all of that, or None; where only an
+    `FP8BlockLinear` reads its result, it hands over codes and block scales (`forward_fp8`) and nothing else is stored."""
+    plain = adapter is None or adapter.merged
+    if norm is not None:
+        if isinstance(base, FP8BlockLinear) and plain and hessian is None:
+            return base.forward_a8(*norm.forward_fp8(x), bias=bias, out=out, out_dtype=torch.float32)
+        x = norm.forward(x)
     if hessian is not None:
         hessian.add(x)
-    if adapter is None or adapter.merged:
+    if isinstance(base, FP8BlockLinear) and plain:
+        return base.forward(x, bias=bias, out=out, out_dtype=torch.float32)
+    if plain:
         return base.forward(x, bias=bias, out=out) if bias is not None or out is not None else base.forward(x)
     return adapter.forward_with(base, x, bias=bias, out=out)

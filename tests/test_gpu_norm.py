@@ -172,6 +172,41 @@ def test_nothing_and_refusals():
         norm.forward(y.cpu())
 
 
+def test_projection_with_a_norm_and_an_adapter():
+    """`proj_fwd` with a norm: over a block-scaled layer the norm hands over codes, beside an adapter it hands over its
+    values; every other layer reads the values too."""
+    from noeira_amd.lora import LoRAAdapter, proj_fwd
+    from noeira_amd.qlinear import QLinear
+
+    norm, x, gen = inputs(21, 960, torch.float32, 4)
+    lin = FP8BlockLinear(960, 320)
+    wq, ws = R.random_weight(gen, 320, 960)
+    lin.set_weight(wq, ws)
+    w, bias = R.matrix(wq, ws), torch.randn(320, generator=gen).cuda()
+    codes, scales = norm.forward_fp8(x)
+    got = proj_fwd(lin, x, bias=bias, norm=norm)
+    assert got.dtype == torch.float32 and torch.equal(got, lin.forward_a8(codes, scales, bias=bias, out_dtype=torch.float32))
+    assert torch.equal(proj_fwd(lin, x), lin.forward(x, out_dtype=torch.float32))
+
+    ad = LoRAAdapter(960, 320, 8, alpha=4.0)
+    a, b = torch.randn(960, 8, generator=gen) * 0.05, torch.randn(8, 320, generator=gen) * 0.05
+    ad.set_params(a.numpy(), b.numpy())
+    xn = norm.forward(x)
+    base = lin.forward(xn, bias=bias, out_dtype=torch.float32)
+    got = proj_fwd(lin, x, adapter=ad, bias=bias, norm=norm)
+    share = 0.5 * (xn.double() @ a.cuda().double()) @ b.cuda().double()
+    mag = 0.5 * (xn.double().abs() @ a.cuda().double().abs()) @ b.cuda().double().abs()
+    R.assert_within(got, base.double() + share, 1.01 * (960 + 8 + 8) * 2 * R.U * mag + R.U * (got.double().abs() + 1e-30), "adapter")
+    with pytest.raises(NQError, match="fp32"):
+        ad.forward_with(lin, xn, out_dtype=torch.bfloat16)
+    ad.merged = True
+    assert torch.equal(proj_fwd(lin, x, adapter=ad, norm=norm), proj_fwd(lin, x, norm=norm))
+
+    q = QLinear(960, 320)
+    q.set_weight((torch.randn(320, 960, generator=gen) * 0.05).numpy())
+    assert torch.equal(proj_fwd(q, x, norm=norm), q.forward(xn))
+
+
 def test_chain_forward_and_back():
     """Norm into codes, a fused q | k | v style projection, an output gradient back through the projection and the norm:
     each step against 64 bits on the step's own inputs, all of it recorded into a graph and replayed."""
