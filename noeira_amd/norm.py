@@ -6,7 +6,6 @@ launch, the normalised values are never stored).  ``vjp`` is the gradient of its
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional
 
 import numpy as np
@@ -44,11 +43,13 @@ class LayerNorm:
         self.beta.copy_(new[1])
 
     def _rows(self, x: torch.Tensor, what: str) -> int:
-        _check_dev(x, f"LayerNorm.{what}: x", _FLOATS)
-        _check_dev(self.gamma, f"LayerNorm.{what}: gamma")
-        if x.numel() % self.DIM:
-            raise L.NQError(L.NQ_ERR_INVALID, f"LayerNorm.{what}: x has {x.numel()} values, not a multiple of DIM = {self.DIM}")
-        return x.numel() // self.DIM
+        _check_dev(x, what, "x", _FLOATS)
+        if self.gamma.get_device() != x.get_device():
+            raise L.NQError(L.NQ_ERR_INVALID, what + ": x and the norm are on different devices")
+        M = x.numel() // self.DIM
+        if M * self.DIM != x.numel():
+            raise L.NQError(L.NQ_ERR_INVALID, f"{what}: x has {x.numel()} values, not a multiple of DIM = {self.DIM}")
+        return M
 
     def _like(self, x: torch.Tensor, M: int, dtype: torch.dtype) -> torch.Tensor:
         t = torch.empty_like(x, dtype=dtype)
@@ -58,26 +59,26 @@ class LayerNorm:
         M = self._rows(x, what)
         if out is not None:
             out_dtype = out.dtype if out_dtype is None else out_dtype
-            _check_dev(out, f"LayerNorm.{what}: out", out_dtype, M * self.DIM)
+            _check_dev(out, what, "out", out_dtype, M * self.DIM)
         out_dtype = x.dtype if out_dtype is None else out_dtype
         if out_dtype not in _TORCH_DT:
-            raise L.NQError(L.NQ_ERR_INVALID, f"LayerNorm.{what}: y must be fp32 or bf16")
+            raise L.NQError(L.NQ_ERR_INVALID, what + ": y must be fp32 or bf16")
         if out is None:
             out = self._like(x, M, out_dtype)
         mean = torch.empty((M,), dtype=torch.float32, device=x.device) if stats else None
         rstd = torch.empty_like(mean) if stats else None
         L.check(L.lib().nq_layer_norm(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(self.gamma), _dev_ptr(self.beta),
-                                      C.c_float(self.eps), _dev_ptr(out), _TORCH_DT[out_dtype], _dev_ptr(mean), _dev_ptr(rstd),
+                                      self.eps, _dev_ptr(out), _TORCH_DT[out_dtype], _dev_ptr(mean), _dev_ptr(rstd),
                                       M, self.DIM, _stream_ptr()))
         return out, mean, rstd
 
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """y [M, DIM], of x's type unless `out_dtype` (fp32 or bf16) says otherwise; `out` may be x itself."""
-        return self._forward(x, out, out_dtype, False, "forward")[0]
+        return self._forward(x, out, out_dtype, False, "LayerNorm.forward")[0]
 
     def forward_train(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None):
         """(y, mean, rstd): `forward` with the statistics fp32 [M] that ``vjp`` takes."""
-        return self._forward(x, out, out_dtype, True, "forward_train")
+        return self._forward(x, out, out_dtype, True, "LayerNorm.forward_train")
 
     def _forward_fp8(self, x, stats, what):
         M = self._rows(x, what)
@@ -86,36 +87,35 @@ class LayerNorm:
         mean = torch.empty((M,), dtype=torch.float32, device=x.device) if stats else None
         rstd = torch.empty_like(mean) if stats else None
         L.check(L.lib().nq_layer_norm_fp8_block(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(self.gamma), _dev_ptr(self.beta),
-                                                C.c_float(self.eps), _dev_ptr(codes), _dev_ptr(scales), _dev_ptr(mean),
+                                                self.eps, _dev_ptr(codes), _dev_ptr(scales), _dev_ptr(mean),
                                                 _dev_ptr(rstd), M, self.DIM, _stream_ptr()))
         return codes, scales, mean, rstd
 
     def forward_fp8(self, x: torch.Tensor):
         """(codes [M, DIM], scales [M, ceil(DIM/128)]): what ``quantize_rows_fp8_block`` makes of the fp32 result."""
-        return self._forward_fp8(x, False, "forward_fp8")[:2]
+        return self._forward_fp8(x, False, "LayerNorm.forward_fp8")[:2]
 
     def forward_fp8_train(self, x: torch.Tensor):
         """(codes, scales, mean, rstd)."""
-        return self._forward_fp8(x, True, "forward_fp8_train")
+        return self._forward_fp8(x, True, "LayerNorm.forward_fp8_train")
 
     def vjp(self, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, grad_output: torch.Tensor,
             grad_input: Optional[torch.Tensor] = None, params: bool = True):
         """(grad_input [M, DIM] of x's type, dgamma, dbeta fp32 [DIM]) from the forward's input and statistics;
         ``params=False`` (a frozen norm): no sums over the rows, dgamma and dbeta are None."""
-        M = self._rows(x, "vjp")
-        _check_dev(grad_output, "LayerNorm.vjp: grad_output", _FLOATS, M * self.DIM)
-        _check_dev(mean, "LayerNorm.vjp: mean", torch.float32, M)
-        _check_dev(rstd, "LayerNorm.vjp: rstd", torch.float32, M)
+        M = self._rows(x, "LayerNorm.vjp")
+        _check_dev(grad_output, "LayerNorm.vjp", "grad_output", _FLOATS, M * self.DIM)
+        _check_dev(mean, "LayerNorm.vjp", "mean", torch.float32, M)
+        _check_dev(rstd, "LayerNorm.vjp", "rstd", torch.float32, M)
         if grad_input is None:
             grad_input = self._like(x, M, x.dtype)
         else:
-            _check_dev(grad_input, "LayerNorm.vjp: grad_input", _FLOATS, M * self.DIM)
+            _check_dev(grad_input, "LayerNorm.vjp", "grad_input", _FLOATS, M * self.DIM)
         dg = db = ws = None
         n = 0
         if params:
-            dg = torch.empty((self.DIM,), dtype=torch.float32, device=x.device)
-            db = torch.empty_like(dg)
-            n = int(L.lib().nq_layer_norm_grad_workspace_bytes(M, self.DIM))
+            dg, db = torch.empty_like(self.gamma), torch.empty_like(self.gamma)
+            n = L.lib().nq_layer_norm_grad_workspace_bytes(M, self.DIM)
             ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
         L.check(L.lib().nq_layer_norm_grad(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(mean), _dev_ptr(rstd), _dev_ptr(self.gamma),
                                            _dev_ptr(grad_output), _TORCH_DT[grad_output.dtype], _dev_ptr(grad_input),

@@ -29,6 +29,7 @@ Q4_BLOCK = 18
 
 _TORCH_DT = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}
 _FLOATS = tuple(_TORCH_DT)
+_CODES = (torch.float8_e4m3fn, torch.uint8)
 
 
 # (the stream's address without a Stream object around it: 0.3 us a call instead of 2.8)
@@ -57,15 +58,16 @@ def _dev_ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return t.data_ptr() if t is not None else None
 
 
-def _check_dev(t: torch.Tensor, what: str, dtype=None, numel=None):
+def _check_dev(t: torch.Tensor, who: str, name: str, dtype=None, numel=None):
     """A contiguous tensor on the current device (the stream the call goes to is that device's), of this type and size."""
     at = t.get_device()
     if at < 0 or at != _device_now() or not t.is_contiguous():
-        raise L.NQError(L.NQ_ERR_INVALID, what + " must be a contiguous tensor on the current device")
+        raise L.NQError(L.NQ_ERR_INVALID, f"{who}: {name} must be a contiguous tensor on the current device")
     if dtype is not None and t.dtype is not dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
-        raise L.NQError(L.NQ_ERR_INVALID, what + " must be " + " or ".join(str(d) for d in (dtype if isinstance(dtype, tuple) else (dtype,))))
+        names = " or ".join(str(d) for d in (dtype if isinstance(dtype, tuple) else (dtype,)))
+        raise L.NQError(L.NQ_ERR_INVALID, f"{who}: {name} must be {names}")
     if numel is not None and t.numel() != numel:
-        raise L.NQError(L.NQ_ERR_SIZE, f"{what} has {t.numel()} values, expected {numel}")
+        raise L.NQError(L.NQ_ERR_SIZE, f"{who}: {name} has {t.numel()} values, expected {numel}")
     return t
 
 
@@ -435,8 +437,8 @@ class FP8BlockLinear(_Layer):
                 raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.set_weight: codes and scales are both arrays or both tensors")
             if tuple(w_codes.shape) != (self.OUT, self.IN) or tuple(scales.shape) != (self.NB, self.KB):
                 raise L.NQError(L.NQ_ERR_SIZE, what)
-            _check_dev(w_codes, "FP8BlockLinear.set_weight: codes", (torch.uint8, torch.float8_e4m3fn))
-            _check_dev(scales, "FP8BlockLinear.set_weight: scales", torch.float32)
+            _check_dev(w_codes, "FP8BlockLinear.set_weight", "codes", _CODES)
+            _check_dev(scales, "FP8BlockLinear.set_weight", "scales", torch.float32)
             L.check(L.lib().nq_set_weight_fp8_block_dev(self._h, _dev_ptr(w_codes), _dev_ptr(scales), _stream_ptr()))
         else:
             w = np.ascontiguousarray(w_codes, dtype=np.uint8)
@@ -450,11 +452,11 @@ class FP8BlockLinear(_Layer):
     @staticmethod
     def _codes(codes: torch.Tensor, scales: torch.Tensor, K: int, what: str) -> int:
         """Checks quantised rows [M, K] and their scales [M, ceil(K/128)]; returns M."""
-        _check_dev(codes, what + ": the codes", (torch.float8_e4m3fn, torch.uint8))
+        _check_dev(codes, what, "the codes", _CODES)
         M = codes.numel() // K
         if M * K != codes.numel():
             raise L.NQError(L.NQ_ERR_INVALID, f"{what}: the codes are {codes.numel()} values, not a multiple of {K}")
-        _check_dev(scales, what + ": the scales", torch.float32, M * (-(-K // 128)))
+        _check_dev(scales, what, "the scales", torch.float32, M * (-(-K // 128)))
         return M
 
     def forward_a8(self, x_codes, x_scales, bias=None, epilogue="none", out=None, out_dtype=torch.bfloat16):
@@ -468,12 +470,12 @@ class FP8BlockLinear(_Layer):
             bias = self.bias
         b_dt = L.DT_F32
         if bias is not None:
-            _check_dev(bias, "FP8BlockLinear.forward_a8: bias", _FLOATS, self.OUT)
+            _check_dev(bias, "FP8BlockLinear.forward_a8", "bias", _FLOATS, self.OUT)
             b_dt = _TORCH_DT[bias.dtype]
         if out is None:
             out = x_codes.new_empty((M, self.OUT), dtype=out_dtype)
         else:
-            _check_dev(out, "FP8BlockLinear.forward_a8: out", out_dtype, M * self.OUT)
+            _check_dev(out, "FP8BlockLinear.forward_a8", "out", out_dtype, M * self.OUT)
         L.check(L.lib().nq_forward(self._h, x_codes.data_ptr(), L.DT_FP8_E4M3, x_scales.data_ptr(), out.data_ptr(),
                                    _TORCH_DT[out_dtype], M, _dev_ptr(bias), b_dt, L.EPI_RELU if epilogue == "relu" else L.EPI_NONE,
                                    _stream_ptr()))
@@ -496,7 +498,7 @@ class FP8BlockLinear(_Layer):
         if grad_input is None:
             grad_input = gy_codes.new_empty((M, self.IN), dtype=out_dtype)
         else:
-            _check_dev(grad_input, "FP8BlockLinear.vjp_a8: grad_input", out_dtype, M * self.IN)
+            _check_dev(grad_input, "FP8BlockLinear.vjp_a8", "grad_input", out_dtype, M * self.IN)
         L.check(L.lib().nq_grad_input_fp8_block(self._h, _dev_ptr(gy_codes), _dev_ptr(gy_scales), _dev_ptr(grad_input),
                                                 _TORCH_DT[out_dtype], M, _stream_ptr()))
         return grad_input
@@ -703,19 +705,19 @@ def quantize_rows_i8(x: torch.Tensor, q: Optional[torch.Tensor] = None, scales: 
 
 def quantize_rows_fp8_block(x: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None):
     """Per row and block of 128 of K: (e4m3fn codes [M, K], scales fp32 [M, ceil(K/128)]) of an fp32 / bf16 [M, K]."""
-    if x.dtype not in _TORCH_DT or x.dim() != 2 or not x.is_contiguous():
+    if x.dtype not in _TORCH_DT or x.dim() != 2:
         raise L.NQError(L.NQ_ERR_INVALID, "quantize_rows_fp8_block: x must be a contiguous fp32/bf16 [M, K] device tensor")
-    _check_dev(x, "quantize_rows_fp8_block: x")
+    _check_dev(x, "quantize_rows_fp8_block", "x")
     M, K = x.shape
     G = -(-K // 128)
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     else:
-        _check_dev(codes, "quantize_rows_fp8_block: codes", (torch.uint8, torch.float8_e4m3fn), M * K)
+        _check_dev(codes, "quantize_rows_fp8_block", "codes", _CODES, M * K)
     if scales is None:
         scales = x.new_empty((M, G), dtype=torch.float32)
     else:
-        _check_dev(scales, "quantize_rows_fp8_block: scales", torch.float32, M * G)
+        _check_dev(scales, "quantize_rows_fp8_block", "scales", torch.float32, M * G)
     L.check(L.lib().nq_quantize_rows_fp8_block(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(codes), _dev_ptr(scales), M, K,
                                                _stream_ptr()))
     return codes, scales
