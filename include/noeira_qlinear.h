@@ -170,6 +170,10 @@ int64_t nq_device_bytes(nq_handle h);
  * (x_scale = fp32 [M], one per row); FP8_E4M3 for FP8_E4M3 weights
  * (x_scale = fp32 [1]) or FP8_BLOCK weights, which take nothing else (x_scale =
  * fp32 [M, ceil(IN/128)], one per row and block: nq_quantize_rows_fp8_block).
+ * FP8_BLOCK with a bf16 y multiplies the codes on the fp8 matrix cores (a
+ * block's sum is off by at most 2.2e-4 of the sum of its terms' magnitudes, a
+ * fraction of the output's own rounding); with an fp32 y on the bf16 ones, over
+ * the exactly decoded codes, so that the sums are fp32 throughout.
  * x_scale is NULL otherwise.
  * y_dtype: F32 or BF16; I32 with x_dtype I8 returns the raw accumulators
  * (no scale, bias or epilogue).  bias may be NULL; bias_dtype F32 or BF16.

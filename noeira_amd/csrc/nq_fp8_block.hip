@@ -83,6 +83,7 @@ __global__ __launch_bounds__(256) void fp8_block_dequantize_kernel(const uint8_t
 
 // ---- activations --------------------------------------------------------------------------------------------------
 
+// One read and one write of everything: 8192 x 4096 in bf16, 102 MB, 17.6 us = 5.8 TB/s.
 // 16 lanes per block of 128.  VEC (K % 8 == 0): a lane's 8 values are adjacent, 128-bit loads and one 64-bit store;
 // otherwise every 16th value, element by element.
 template <bool BF16, bool VEC>
@@ -135,8 +136,11 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void
 
 // ---- the product --------------------------------------------------------------------------------------------------
 
-// MT x NT MFMA tiles of 16 x 16 per workgroup, the blocks of K dealt over KW wavefronts, whose sums meet in LDS in
-// wavefront order (bit-repeatable).  U: blocks requested together.
+// Few rows: MT x NT MFMA tiles of 16 x 16 per workgroup, the blocks of K dealt over KW wavefronts, whose sums meet in LDS
+// in wavefront order (bit-repeatable).  U: blocks requested together.  Both operands go from memory to registers: the
+// weight's tiles are contiguous, every byte of them is read once per 16 MT rows, and at one row nothing else matters.
+// One row over 4096 -> 11008 (45 MB, rotating over copies): 9.1 us in bf16, 4.9 TB/s (a plain copy moves 5.0); 256 rows over
+// 4096 -> 4096: 17.4 - 19, 134 MB from L2 (8.7 TB/s, which bounds every call from about 16 rows on).
 template <int MT, int NT, int KW, int U, bool EXACT>
 __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockParams p) {
     constexpr int ROWS = 16 * MT, CH = 16 * NT;

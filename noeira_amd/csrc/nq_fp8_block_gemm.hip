@@ -4,6 +4,21 @@
 // A stage of the K loop is one block of 128 k: x tile BM x 128 B, weight tile BN x 128 B and their scales, filled straight
 // from global memory (global_load_lds) into one of NB stage buffers.  A wavefront owns TI x TJ results of 16 x 16, and its
 // channels lie in one block of 128, so its weight scale is one number per stage.
+//
+// Why these tiles.  The scales make every result pass the vector ALU once per block (a product into registers of its own,
+// then four multiply-adds per lane), so the accumulators have to be vector registers: 128 of a wavefront's 256 with two
+// wavefronts per SIMD, 64 x 128 per wavefront, 256 x 256 per CU.  (One wavefront per SIMD with twice the registers could
+// not address twice the accumulators, and left the matrix core waiting on its own multiply-adds: 31 us against 24 for
+// 512 rows over 4096 -> 4096 on 128 x 128 tiles.)  Smaller calls take smaller tiles (estimate() below).
+//
+// What bounds it, 8192 x 4096 x 4096 in bf16: 119 - 126 us = 2.2 - 2.3 PFLOP/s, what this library's GEMM with one scale per
+// tensor takes on the same boxes (120 us) - the board's power limit.  Below that limit (128 workgroups; parts taken out one
+// at a time): whole 50 us; without the transfers 42, without the multiply-adds 44, without either 38, the products alone
+// 33 (their matrix core time).  The transfers cost what they occupy of LDS (64 KiB in, 192 KiB of fragments out per stage:
+// 2048 cycles at 128 B, as many as the products), the multiply-adds about half of their 1024 vector cycles per stage and
+// SIMD.  On 128 x 128 tiles LDS is the bound outright (128 KiB per 512 cycles of products: 0.47 us a stage; 18.2 - 20.6 us
+// a round at K = 4096).  With an fp32 y the two bf16 products per fp8 one and 16 conversions per fragment take 239 us
+// (1.15 PFLOP/s; a library bf16 product of the same size 232).
 #include "nq_fp8_block.h"
 
 namespace nq {
@@ -155,11 +170,12 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     // long delivered them.
     //
     // The transfers stand between the products, spread out: the CU's address unit takes about 22 cycles for each, and a
-    // wavefront that finds it busy waits with its products behind it (all of a stage's in its last pair: XXX).  With three
-    // buffers and more, stage st requests stage st + NB - 1 into the buffer that the last barrier freed.  With two, that
-    // would leave a stage's last transfers no time to land; there the two halves of the buffer are freed one after the
-    // other: the x half by a barrier behind the first pair (the token fragments are in registers by then), refilled during
-    // the middle pairs, the w half by the stage's own barrier, refilled during its last pair and the next one's first.
+    // wavefront that finds it busy waits with its products behind it (all of a stage's in its last pair: 2 us of 52 on 128
+    // workgroups of 256 x 256).  With three buffers and more, stage st requests stage st + NB - 1 into the buffer that the
+    // last barrier freed.  With two, that would leave a stage's last transfers no time to land; there the two halves of
+    // the buffer are freed one after the other: the x half by a barrier behind the first pair (the token fragments are in
+    // registers by then), refilled during the middle pairs, the w half by the stage's own barrier, refilled during its
+    // last pair and the next one's first.
     constexpr int Q = TI * TJ, QB = Q - 2 * TI;  // products of a stage; the first one behind its barrier
     constexpr int T = DX + DW;
     constexpr int AHEAD = NB >= 3 ? NB - 1 : 2;  // stages requested before the first
