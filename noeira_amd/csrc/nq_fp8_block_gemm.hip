@@ -245,7 +245,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             }
             if constexpr (NB == 2 && pr == 1 && !LAST) {
                 if (more) {
-                    asm volatile("" ::: "memory");
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wavefront's token fragments are in registers
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
                 }

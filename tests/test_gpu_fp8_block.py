@@ -112,7 +112,9 @@ SHAPES = [(1, 16, 1), (1, 128, 16), (1, 960, 2560), (1, 4096, 1040), (2, 272, 12
           (17, 960, 320), (33, 1024, 100), (64, 2560, 960), (65, 2064, 700), (100, 3200, 512), (135, 960, 2567), (256, 960, 2560),
           (257, 512, 384), (300, 4096, 1040), (513, 1040, 257), (700, 640, 1300), (1024, 1024, 2048),
           # a hundred tiles of 256 x 256 and more: one block of K, part of one, two, an odd and an even number of them
-          (2100, 128, 4100), (3000, 16, 2832), (2049, 256, 4104), (2304, 656, 4001), (4096, 1024, 2048)]
+          (2100, 128, 4100), (3000, 16, 2832), (2049, 256, 4104), (2304, 656, 4001), (4096, 1024, 2048),
+          # the other tiles of the GEMM, and tiles left over after the last full round
+          (500, 496, 4001), (1000, 512, 4000), (2045, 528, 4090), (4093, 272, 4345)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
