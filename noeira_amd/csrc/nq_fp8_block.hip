@@ -25,7 +25,7 @@
 #include "nq_fp8_block.h"
 #include "nq_fp8_quant.h"
 
-#include <type_traits>
+#include <algorithm>
 
 namespace nq {
 
@@ -90,48 +90,49 @@ template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void* __restrict__ x, uint8_t* __restrict__ codes,
                                                                       float* __restrict__ scales, int32_t K, uint32_t G,
                                                                       uint32_t blocks) {
-    const uint32_t b = blockIdx.x * 16u + (threadIdx.x >> 4);
-    if (b >= blocks) return;  // (16 lanes leave together: a DPP row)
-    const uint32_t m = b / G, g = b - m * G;
     const int l = threadIdx.x & 15;
-    const int64_t base = (int64_t)m * K;
-    float v[8];
-    float s;
-    if constexpr (VEC) {
-        const int32_t k = (int32_t)g * 128 + 8 * l;
-        const bool in = k < K;
+    // (16 lanes, a DPP row, enter and leave together; more than one turn only beyond 2^24 workgroups)
+    for (uint32_t b = blockIdx.x * 16u + (threadIdx.x >> 4); b < blocks; b += gridDim.x * 16u) {
+        const uint32_t m = b / G, g = b - m * G;
+        const int64_t base = (int64_t)m * K;
+        float v[8];
+        float s;
+        if constexpr (VEC) {
+            const int32_t k = (int32_t)g * 128 + 8 * l;
+            const bool in = k < K;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 0.0f;
-        if (in) {
-            if constexpr (BF16) {
-                const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + base + k);
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            for (int i = 0; i < 8; i++) v[i] = 0.0f;
+            if (in) {
+                if constexpr (BF16) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + base + k);
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-            } else {
-                const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + base + k);
-                const float4 a = p[0], c = p[1];
-                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = c.x, v[5] = c.y, v[6] = c.z, v[7] = c.w;
+                    for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+                } else {
+                    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + base + k);
+                    const float4 a = p[0], c = p[1];
+                    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = c.x, v[5] = c.y, v[6] = c.z, v[7] = c.w;
+                }
+            }
+            const uint2 q = quantize_block16(v, s);
+            if (in) *reinterpret_cast<uint2*>(codes + base + k) = q;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int32_t k = (int32_t)g * 128 + 16 * i + l;
+                v[i] = k >= K ? 0.0f
+                              : BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(x)[base + k] << 16)
+                                     : reinterpret_cast<const float*>(x)[base + k];
+            }
+            const uint2 q = quantize_block16(v, s);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int32_t k = (int32_t)g * 128 + 16 * i + l;
+                if (k < K) codes[base + k] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
             }
         }
-        const uint2 q = quantize_block16(v, s);
-        if (in) *reinterpret_cast<uint2*>(codes + base + k) = q;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int32_t k = (int32_t)g * 128 + 16 * i + l;
-            v[i] = k >= K ? 0.0f
-                          : BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(x)[base + k] << 16)
-                                 : reinterpret_cast<const float*>(x)[base + k];
-        }
-        const uint2 q = quantize_block16(v, s);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int32_t k = (int32_t)g * 128 + 16 * i + l;
-            if (k < K) codes[base + k] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
-        }
+        if (l == 0) scales[b] = s;
     }
-    if (l == 0) scales[b] = s;
 }
 
 // ---- the product --------------------------------------------------------------------------------------------------
@@ -337,7 +338,7 @@ int32_t launch_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* 
     if (blocks > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: more than 2^31 - 1 blocks of 128");
     const bool bf16 = x_dtype == NQ_DT_BF16, vec = K % 8 == 0;
 #define NQ_QB(B, V)                                                                                                        \
-    hipLaunchKernelGGL((quantize_rows_fp8_block_kernel<B, V>), dim3((unsigned)((blocks + 15) / 16)), dim3(256), 0, s, x,   \
+    hipLaunchKernelGGL((quantize_rows_fp8_block_kernel<B, V>), dim3((unsigned)std::min<int64_t>((blocks + 15) / 16, (1 << 24) - 1)), dim3(256), 0, s, x, \
                        codes, scales, K, (uint32_t)G, (uint32_t)blocks)
     if (bf16 && vec) NQ_QB(true, true);
     else if (bf16) NQ_QB(true, false);
@@ -350,6 +351,10 @@ int32_t launch_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* 
 
 int32_t launch_fp8_block(const ForwardArgs& a) {
     const nq_layer* L = a.L;
+    int device = -1;
+    NQ_HIP(hipGetDevice(&device));
+    if (device != L->device)
+        return fail(NQ_ERR_INVALID, "layer was loaded on device " + std::to_string(L->device) + " but the current device is " + std::to_string(device));
     BlockParams p{};
     p.x = reinterpret_cast<const uint8_t*>(a.x), p.w = L->d_codes;
     p.xs = a.x_scale, p.ws = reinterpret_cast<const float*>(L->d_scales), p.bias = a.bias;

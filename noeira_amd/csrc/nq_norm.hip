@@ -223,38 +223,40 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const Nor
 // rows beyond 16384 values: one workgroup per row, three passes (the row comes from the caches after the first)
 __global__ __launch_bounds__(1024) void layer_norm_long_kernel(const NormArgs a) {
     __shared__ float lds[2][16];
-    const int64_t m = blockIdx.x, base = m * a.D;
     const int wave = threadIdx.x / 64;
-    float sum = 0.0f;
-    for (int64_t d = threadIdx.x; d < a.D; d += 1024) sum += load1(a.x, a.x_dtype, base + d);
-    const float mean = team_sum<1024>(sum, lds[0], wave) / (float)a.D;
-    float sq = 0.0f;
-    for (int64_t d = threadIdx.x; d < a.D; d += 1024) {
-        const float t = load1(a.x, a.x_dtype, base + d) - mean;
-        sq += t * t;
-    }
-    const float rstd = 1.0f / sqrtf(team_sum<1024>(sq, lds[1], wave) / (float)a.D + a.eps);
-    if (threadIdx.x == 0 && a.mean) a.mean[m] = mean, a.rstd[m] = rstd;
-    for (int64_t d0 = 0; d0 < a.D; d0 += 8192) {
-        const int64_t k = d0 + (int64_t)(threadIdx.x / 16) * 128 + threadIdx.x % 16;  // every 16th value of a block
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int64_t d = k + 16 * i;
-            f[i] = 0.0f;
-            if (d < a.D) f[i] = (load1(a.x, a.x_dtype, base + d) - mean) * rstd * (a.gamma ? a.gamma[d] : 1.0f) + (a.beta ? a.beta[d] : 0.0f);
+    for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
+        const int64_t base = m * a.D;
+        float sum = 0.0f;
+        for (int64_t d = threadIdx.x; d < a.D; d += 1024) sum += load1(a.x, a.x_dtype, base + d);
+        const float mean = team_sum<1024>(sum, lds[0], wave) / (float)a.D;
+        float sq = 0.0f;
+        for (int64_t d = threadIdx.x; d < a.D; d += 1024) {
+            const float t = load1(a.x, a.x_dtype, base + d) - mean;
+            sq += t * t;
         }
-        if (a.y) {
+        const float rstd = 1.0f / sqrtf(team_sum<1024>(sq, lds[1], wave) / (float)a.D + a.eps);
+        if (threadIdx.x == 0 && a.mean) a.mean[m] = mean, a.rstd[m] = rstd;
+        for (int64_t d0 = 0; d0 < a.D; d0 += 8192) {
+            const int64_t k = d0 + (int64_t)(threadIdx.x / 16) * 128 + threadIdx.x % 16;  // every 16th value of a block
+            float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (k + 16 * i < a.D) store1(a.y, a.y_dtype, base + k + 16 * i, f[i]);
-        } else {
-            float s;
-            const uint2 q = quantize_block16(f, s);
+            for (int i = 0; i < 8; i++) {
+                const int64_t d = k + 16 * i;
+                f[i] = 0.0f;
+                if (d < a.D) f[i] = (load1(a.x, a.x_dtype, base + d) - mean) * rstd * (a.gamma ? a.gamma[d] : 1.0f) + (a.beta ? a.beta[d] : 0.0f);
+            }
+            if (a.y) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (k + 16 * i < a.D) a.codes[base + k + 16 * i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
-            if (threadIdx.x % 16 == 0 && k < a.D) a.scales[m * ((a.D - 1) / 128 + 1) + k / 128] = s;
+                for (int i = 0; i < 8; i++)
+                    if (k + 16 * i < a.D) store1(a.y, a.y_dtype, base + k + 16 * i, f[i]);
+            } else {
+                float s;
+                const uint2 q = quantize_block16(f, s);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (k + 16 * i < a.D) a.codes[base + k + 16 * i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+                if (threadIdx.x % 16 == 0 && k < a.D) a.scales[m * ((a.D - 1) / 128 + 1) + k / 128] = s;
+            }
         }
     }
 }
@@ -377,20 +379,22 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(const NormGradArg
 // rows beyond 16384 values: gx, one workgroup per row, two passes
 __global__ __launch_bounds__(1024) void layer_norm_grad_x_long_kernel(const NormGradArgs a) {
     __shared__ float lds[2][16];
-    const int64_t m = blockIdx.x, base = m * a.D;
     const int wave = threadIdx.x / 64;
-    const float mean = a.mean[m], rstd = a.rstd[m];
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int64_t d = threadIdx.x; d < a.D; d += 1024) {
-        const float t = load1(a.gy, a.gy_dtype, base + d) * (a.gamma ? a.gamma[d] : 1.0f);
-        s1 += t;
-        s2 += t * ((load1(a.x, a.x_dtype, base + d) - mean) * rstd);
-    }
-    const float c1 = team_sum<1024>(s1, lds[0], wave) / (float)a.D, c2 = team_sum<1024>(s2, lds[1], wave) / (float)a.D;
-    for (int64_t d = threadIdx.x; d < a.D; d += 1024) {
-        const float t = load1(a.gy, a.gy_dtype, base + d) * (a.gamma ? a.gamma[d] : 1.0f);
-        const float xh = (load1(a.x, a.x_dtype, base + d) - mean) * rstd;
-        store1(a.gx, a.gx_dtype, base + d, rstd * (t - c1 - xh * c2));
+    for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
+        const int64_t base = m * a.D;
+        const float mean = a.mean[m], rstd = a.rstd[m];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int64_t d = threadIdx.x; d < a.D; d += 1024) {
+            const float t = load1(a.gy, a.gy_dtype, base + d) * (a.gamma ? a.gamma[d] : 1.0f);
+            s1 += t;
+            s2 += t * ((load1(a.x, a.x_dtype, base + d) - mean) * rstd);
+        }
+        const float c1 = team_sum<1024>(s1, lds[0], wave) / (float)a.D, c2 = team_sum<1024>(s2, lds[1], wave) / (float)a.D;
+        for (int64_t d = threadIdx.x; d < a.D; d += 1024) {
+            const float t = load1(a.gy, a.gy_dtype, base + d) * (a.gamma ? a.gamma[d] : 1.0f);
+            const float xh = (load1(a.x, a.x_dtype, base + d) - mean) * rstd;
+            store1(a.gx, a.gx_dtype, base + d, rstd * (t - c1 - xh * c2));
+        }
     }
 }
 // ... and the partials: one thread per column and slice of rows
@@ -518,7 +522,7 @@ int32_t launch_grad_held(const NormGradArgs& a, int32_t P, hipStream_t s) {
 
 int32_t launch_layer_norm(const NormArgs& a, hipStream_t s) {
     if (a.D > MAX_HELD) {
-        hipLaunchKernelGGL(layer_norm_long_kernel, dim3((unsigned)a.M), dim3(1024), 0, s, a);
+        hipLaunchKernelGGL(layer_norm_long_kernel, dim3((unsigned)std::min(a.M, 1 << 20)), dim3(1024), 0, s, a);
         NQ_HIP(hipGetLastError());
         return NQ_OK;
     }
@@ -549,7 +553,7 @@ int32_t launch_layer_norm_grad(const NormGradArgs& a, hipStream_t s) {
             hipLaunchKernelGGL(layer_norm_grad_w_long_kernel, dim3((unsigned)((a.D - 1) / 64 + 1), (unsigned)P), dim3(64), 0, s, a);
             NQ_HIP(hipGetLastError());
         }
-        hipLaunchKernelGGL(layer_norm_grad_x_long_kernel, dim3((unsigned)a.M), dim3(1024), 0, s, a);
+        hipLaunchKernelGGL(layer_norm_grad_x_long_kernel, dim3((unsigned)std::min(a.M, 1 << 20)), dim3(1024), 0, s, a);
         NQ_HIP(hipGetLastError());
     } else {
         const int32_t rc = launch_grad_held(a, P, s);

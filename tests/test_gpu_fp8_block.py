@@ -327,6 +327,33 @@ def test_from_linear():
     R.assert_within(lin.forward(x, out_dtype=torch.float32), y, R.product_bound(xv, wv, y, bv, torch.float32), "from_linear")
 
 
+# ---- offsets beyond 32 bits -----------------------------------------------------------------------------------------
+
+
+def test_rows_and_outputs_beyond_four_gigabytes():
+    """The last rows of calls whose codes, or whose outputs, end beyond 2^32 bytes."""
+    gen = torch.Generator().manual_seed(12)
+    for M, K, N, dtype in ((1048583, 4112, 24, torch.bfloat16), (140009, 144, 8200, torch.float32)):
+        wq, ws = R.random_weight(gen, N, K)
+        lin = layer(wq, ws)
+        xq = torch.zeros((M, K), dtype=torch.uint8, device="cuda")
+        xs = torch.ones((M, -(-K // 128)), device="cuda")
+        tail = R.random_rows(gen, 70, K)
+        xq[-70:], xs[-70:] = tail
+        assert max(xq.numel(), M * N * torch.finfo(dtype).bits // 8) > 2 ** 32
+        y = lin.forward_a8(xq, xs, out_dtype=dtype)
+        assert not y[:-70].any()
+        x, w = R.rows(*tail), R.matrix(wq, ws)
+        R.assert_within(y[-70:], x @ w.t(), R.product_bound(x, w, x @ w.t(), None, dtype), "last rows")
+        del y, xq
+    x = torch.zeros((2097169, 1040), dtype=torch.bfloat16, device="cuda")
+    x[-9:] = torch.randn(9, 1040, generator=gen).to(torch.bfloat16).cuda()
+    codes, scales = quantize_rows_fp8_block(x)
+    want = quantize_rows_fp8_block(x[-9:].contiguous())
+    assert torch.equal(bits(codes[-9:]), bits(want[0])) and torch.equal(scales[-9:], want[1])
+    assert not codes[:-9].view(torch.uint8).any() and (scales[:-9] == 1).all()
+
+
 # ---- streams, graphs ------------------------------------------------------------------------------------------------
 
 

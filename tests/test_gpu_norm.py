@@ -84,6 +84,29 @@ def test_constant_rows_and_far_means(D):
     R.assert_within(norm.forward(far), want, e_y, "far mean")
 
 
+@pytest.mark.parametrize("D", [1040, 16400])
+def test_rows_beyond_four_gigabytes(D):
+    """The last rows of a call whose rows end beyond 2^32 bytes have the bits of a call of their own."""
+    M = 2 ** 31 // D + 100
+    norm, _, gen = inputs(1, D, torch.bfloat16)
+    x = torch.ones((M, D), dtype=torch.bfloat16, device="cuda")
+    x[-9:] = torch.randn(9, D, generator=gen).to(torch.bfloat16).cuda()
+    own = x[-9:].clone()
+    y, mean, rstd = norm.forward_train(x)
+    want = norm.forward_train(own)
+    assert torch.equal(y[-9:], want[0]) and torch.equal(mean[-9:], want[1]) and torch.equal(rstd[-9:], want[2])
+    assert torch.equal(y[0], norm.beta.to(torch.bfloat16))
+    codes, scales = norm.forward_fp8(x)
+    wq, wsc = norm.forward_fp8(own)
+    assert torch.equal(codes[-9:].view(torch.uint8), wq.view(torch.uint8)) and torch.equal(scales[-9:], wsc)
+    gy = torch.zeros_like(x)
+    gy[-9:] = 1.0
+    gx, dg, db = norm.vjp(x, mean, rstd, gy)
+    wx, wg, wb = norm.vjp(own, want[1], want[2], torch.ones_like(own))
+    assert torch.equal(gx[-9:], wx) and not gx[:-9].any()
+    assert torch.equal(db, wb) and torch.allclose(dg, wg, rtol=0, atol=20 * 9 * R.U * 8)  # nine terms below 8 in another order
+
+
 def test_non_finite_rows_stay_alone():
     norm, x, _ = inputs(6, 960, torch.float32)
     clean = norm.forward(x)
