@@ -390,6 +390,7 @@ static int32_t set_weight_fp8_block(nq_handle h, const uint8_t* codes, const flo
     if (h->format != NQ_FMT_FP8_BLOCK)
         return fail(NQ_ERR_INVALID, "nq_set_weight_fp8_block: the layer's format is not FP8_BLOCK");
     if (!codes || !scales) return fail(NQ_ERR_INVALID, "nq_set_weight_fp8_block: null codes or scales");
+    if ((uintptr_t)scales & 3) return fail(NQ_ERR_INVALID, "nq_set_weight_fp8_block: scales must be 4-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     h->loaded = false;
     if ((rc = bind_device(h))) return rc;
@@ -1417,6 +1418,7 @@ int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, co
                            const void* gy, int32_t gy_dtype, void* gx, int32_t gx_dtype, float* dgamma, float* dbeta,
                            int32_t M, int32_t D, void* workspace, int64_t workspace_bytes, void* stream) {
     if (M < 0 || D <= 0) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: M >= 0 and D > 0 are required");
+    if (D > 1 << 26) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: rows of more than 2^26 values");
     for (int32_t t : {x_dtype, gy_dtype, gx_dtype})
         if (t != NQ_DT_F32 && t != NQ_DT_BF16) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: x, gy and gx must be fp32 or bf16");
     if ((dgamma == nullptr) != (dbeta == nullptr))

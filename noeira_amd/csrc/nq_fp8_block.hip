@@ -264,7 +264,7 @@ template <int MT, int NT, int KW, int U>
 int32_t launch_tile(BlockParams p, hipStream_t s) {
     p.tiles_m = (p.M + 16 * MT - 1) / (16 * MT);
     const int64_t grid = (int64_t)p.tiles_m * ((p.N + 16 * NT - 1) / (16 * NT));
-    if (grid > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
+    if (grid * 64 * KW > UINT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
     constexpr size_t lds = sizeof(float) * KW * 16 * MT * (16 * NT + 4);
     static LdsAttrOnce attr[2];
     if (p.y_dtype == NQ_DT_F32) {

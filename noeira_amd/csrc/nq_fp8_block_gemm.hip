@@ -12,7 +12,7 @@
 // 512 rows over 4096 -> 4096 on 128 x 128 tiles.)  Smaller calls take smaller tiles (estimate() below).
 //
 // What bounds it, 8192 x 4096 x 4096 in bf16: 119 - 126 us = 2.2 - 2.3 PFLOP/s, what this library's GEMM with one scale per
-// tensor takes on the same boxes (120 us) - the board's power limit.  Below that limit (128 workgroups; parts taken out one
+// tensor takes (120 us) - the board's power limit.  Below that limit (128 workgroups; parts taken out one
 // at a time): whole 50 us; without the transfers 42, without the multiply-adds 44, without either 38, the products alone
 // 33 (their matrix core time).  The transfers cost what they occupy of LDS (64 KiB in, 192 KiB of fragments out per stage:
 // 2048 cycles at 128 B, as many as the products), the multiply-adds about half of their 1024 vector cycles per stage and

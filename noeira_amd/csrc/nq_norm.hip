@@ -182,16 +182,16 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const Nor
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             const int k = first_index<T, VEC>(t, v);
+            const float centre = !VEC || k < a.D ? mean : 0.0f;
             float part = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                f[v][i] -= mean;
-                if constexpr (VEC)
-                    part = fmaf(f[v][i], f[v][i], part);
-                else
-                    part += k + 16 * i < a.D ? f[v][i] * f[v][i] : 0.0f;
+                // (zeros behind the row stay zeros: a mean beyond 2^128 / rstd would make them infinite below, and those a
+                // NaN in the last block's largest magnitude)
+                f[v][i] = VEC || k + 16 * i < a.D ? f[v][i] - centre : 0.0f;
+                part = VEC ? fmaf(f[v][i], f[v][i], part) : part + f[v][i] * f[v][i];
             }
-            sq += !VEC || k < a.D ? part : 0.0f;
+            sq += part;
         }
         const float rstd = 1.0f / sqrtf(team_sum<T>(sq, lds[1], wave) / d + a.eps);
         if (a.mean && t == 0) a.mean[m] = mean, a.rstd[m] = rstd;
@@ -286,6 +286,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(const NormGradArg
     float mean = 0.0f, rstd = 0.0f;
     auto request = [&](int64_t row) {
         const int end = row < a.M ? a.D : 0;  // (a team without a row left takes part in the barriers with zeros)
+        rstd = 0.0f;
         if (row < a.M) mean = a.mean[row], rstd = a.rstd[row];
 #pragma unroll
         for (int v = 0; v < NV; v++) {
@@ -311,11 +312,13 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(const NormGradArg
         for (int v = 0; v < NV; v++) {
             widen<XB>(cx[v], xh[v]);
             widen<GB>(cg[v], f[v]);
+            const int at = first_index<T, VEC>(t, v);
+            const float rv = !VEC || at < a.D ? rs : 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                // (behind the row gy is zero, so that nothing of xh counts there; a team without a row keeps its last
-                // statistics, and has gy = 0 everywhere)
-                xh[v][i] = (xh[v][i] - mean) * rs;
+                // (behind the row, and for a team without one, gy is zero and rstd counts as zero: a mean beyond
+                // 2^128 / rstd times that zero would be a NaN in every sum)
+                xh[v][i] = VEC || at + 16 * i < a.D ? (xh[v][i] - mean) * rv : 0.0f;
                 dg[v][i] += f[v][i] * xh[v][i];
                 db[v][i] += f[v][i];
                 f[v][i] *= w[v][i];

@@ -70,6 +70,10 @@ class LoRAAdapter:
         call runs on the kernel that keeps its rows' activations resident, the two of `forward` + `forward_add`
         elsewhere.  B = 0 returns the bits of ``base.forward(x)``."""
         if isinstance(base, FP8BlockLinear):  # its kernels read codes, the adapter the activations themselves: two steps
+            if self.merged:
+                return base.forward(x, bias=bias, out=out, out_dtype=out_dtype)
+            if base.IN != self.IN or base.OUT != self.OUT:
+                raise L.NQError(L.NQ_ERR_INVALID, "LoRAAdapter.forward_with: the adapter and the base layer differ in shape")
             if out_dtype != torch.float32:
                 raise L.NQError(L.NQ_ERR_UNSUPPORTED, "LoRAAdapter.forward_with: an adapter beside an FP8BlockLinear adds into fp32")
             y = base.forward(x, bias=bias, out=out, out_dtype=torch.float32)

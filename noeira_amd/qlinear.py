@@ -452,6 +452,8 @@ class FP8BlockLinear(_Layer):
     @staticmethod
     def _codes(codes: torch.Tensor, scales: torch.Tensor, K: int, what: str) -> int:
         """Checks quantised rows [M, K] and their scales [M, ceil(K/128)]; returns M."""
+        if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+            raise L.NQError(L.NQ_ERR_INVALID, what + ": e4m3 codes and their scales (quantize_rows_fp8_block) are needed")
         _check_dev(codes, what, "the codes", _CODES)
         M = codes.numel() // K
         if M * K != codes.numel():
@@ -562,6 +564,10 @@ class FusedRows:
         M = _check_x(x, self.IN, "FusedRows.forward")
         if self._kind is FP8BlockLinear:
             FP8BlockLinear._codes(x, x_scale, self.IN, "FusedRows.forward")
+            for o, n in zip(outs or (), self.OUTS):
+                _check_dev(o, "FusedRows.forward", "an output", out_dtype, M * n)
+            if bias is not None:
+                _check_dev(bias, "FusedRows.forward", "bias", _FLOATS, self.OUT)
         if outs is None:
             outs = [torch.empty((M, n), dtype=out_dtype, device=x.device) for n in self.OUTS]
         y_dt = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16}[out_dtype]

@@ -42,6 +42,7 @@ def test_before_a_weight_is_set():
     refuses(lib.nq_grad_input_fp8_block(None, one, one, one, L.DT_F32, 1, None), L.NQ_ERR_INVALID, "null layer handle")
     refuses(lib.nq_set_weight_fp8_block(h, None, None, None), L.NQ_ERR_INVALID, "null codes or scales")
     refuses(lib.nq_set_weight_fp8_block_dev(h, None, one, None), L.NQ_ERR_INVALID, "null codes or scales")
+    refuses(lib.nq_set_weight_fp8_block_dev(h, one, P(66), None), L.NQ_ERR_INVALID, "4-byte aligned")
     refuses(lib.nq_set_weight_fp8(h, one, 1.0, None), L.NQ_ERR_INVALID, "not FP8_E4M3")
     rc, other = create(128, 64, fmt=L.FMT_FP8_E4M3)
     refuses(lib.nq_set_weight_fp8_block(other, one, one, None), L.NQ_ERR_INVALID, "not FP8_BLOCK")
@@ -100,7 +101,7 @@ GRAD = dict(x=64, xdt=L.DT_F32, mean=64, rstd=64, gamma=64, gy=128, gydt=L.DT_F3
 
 
 @pytest.mark.parametrize("change,code,words", [
-    (dict(D=0), L.NQ_ERR_INVALID, "M >= 0 and D > 0"), (dict(gydt=L.DT_I8), L.NQ_ERR_INVALID, "must be fp32 or bf16"),
+    (dict(D=0), L.NQ_ERR_INVALID, "M >= 0 and D > 0"), (dict(D=2 ** 26 + 1), L.NQ_ERR_INVALID, "2^26"), (dict(gydt=L.DT_I8), L.NQ_ERR_INVALID, "must be fp32 or bf16"),
     (dict(gxdt=7), L.NQ_ERR_INVALID, "must be fp32 or bf16"), (dict(dg=None), L.NQ_ERR_INVALID, "together"),
     (dict(dg=66), L.NQ_ERR_INVALID, "4-byte"), (dict(gy=None), L.NQ_ERR_INVALID, "null pointer"),
     (dict(mean=None), L.NQ_ERR_INVALID, "null pointer"), (dict(gx=196), L.NQ_ERR_INVALID, "16-byte"),

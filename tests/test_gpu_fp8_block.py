@@ -138,6 +138,43 @@ def test_product(M, K, N, dtype):
         R.assert_within(got, z.clamp(min=0), R.product_bound(x, w, z, bias.double(), dtype), "bias and ReLU")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(3, 272, 132), (40, 960, 129), (300, 512, 260), (700, 144, 1001), (1100, 256, 2560), (2100, 128, 4100)])
+def test_output_that_begins_on_four_bytes(M, K, N, dtype):
+    """An output 4 but not 16 bytes aligned gets the aligned one's bits, and nothing beside it is written."""
+    gen = torch.Generator().manual_seed(M + N)
+    xq, xs = R.random_rows(gen, M, K)
+    lin = layer(*R.random_weight(gen, N, K))
+    want = lin.forward_a8(xq, xs, out_dtype=dtype)
+    first = 4 // want.element_size()
+    store = torch.full((M * N + 64,), 77.0, dtype=dtype, device="cuda")
+    lin.forward_a8(xq, xs, out=store[first: first + M * N].view(M, N), out_dtype=dtype)
+    assert torch.equal(bits(store[first: first + M * N].view(M, N)), bits(want))
+    assert (store[:first] == 77.0).all() and (store[first + M * N:] == 77.0).all()
+
+
+def test_weights_set_again():
+    """A second set of weights, from the device or the host, replaces the first, W^T with it; dropping the logical bytes
+    leaves the layer running."""
+    gen = torch.Generator().manual_seed(8)
+    xq, xs = R.random_rows(gen, 70, 272)
+    gq, gs = R.random_rows(gen, 70, 144)
+    lin = FP8BlockLinear(272, 144, grad=True)
+    for turn in range(4):
+        wq, ws = R.random_weight(gen, 144, 272)
+        if turn % 2:
+            lin.set_weight(wq.cpu().numpy(), ws.cpu().numpy())
+            L.check(L.lib().nq_keep_only_repacked(lin._h))
+        else:
+            lin.set_weight(wq, ws)
+        x, g, w = R.rows(xq, xs), R.rows(gq, gs), R.matrix(wq, ws)
+        R.assert_within(lin.forward_a8(xq, xs, out_dtype=torch.float32), x @ w.t(), R.product_bound(x, w, x @ w.t(), None, torch.float32), "y")
+        R.assert_within(lin.vjp_a8(gq, gs), g @ w, R.product_bound(g, w.t(), g @ w, None, torch.float32), "gx")
+    buf = np.empty(144 * 272, np.uint8)
+    with pytest.raises(NQError, match="no blocks are kept"):
+        L.check(L.lib().nq_get_blocks(lin._h, buf.ctypes.data, buf.size))
+
+
 def test_dequantize_and_device_bytes():
     gen = torch.Generator().manual_seed(3)
     for N, K in ((1, 16), (129, 272), (300, 960)):
@@ -209,6 +246,8 @@ def test_nothing_and_refusals():
         lin.forward_a8(xq, xs.t())
     with pytest.raises(NQError, match="expected 192"):
         lin.forward_a8(xq, xs, out=torch.empty((3, 48), dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(NQError, match="are needed"):
+        lin.forward_a8(xq, None)
     with pytest.raises(NQError, match="epilogue"):
         lin.forward_a8(xq, xs, epilogue="swiglu")
     with pytest.raises(NQError, match="bias has 47 values"):
@@ -255,6 +294,45 @@ def test_fused_rows(M):
     assert torch.equal(fused_dequantized(fused, 712, 960), whole.float())
     with pytest.raises(NQError):
         fused.forward(xq, xs[:, :7].contiguous())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("M", [1100, 2200])
+def test_fused_rows_of_a_batch(M, dtype):
+    """Rows enough that the parts run one after the other on the GEMM (2200; 1100 in one launch of the few-rows kernel,
+    whose sums meet in another order than a part's own): values of the parts, with a bias across all of them."""
+    gen = torch.Generator().manual_seed(2)
+    parts = [R.random_weight(gen, n, 1040) for n in (2048, 1024, 1030)]
+    fused = FusedRows([layer(*p) for p in parts])
+    xq, xs = R.random_rows(gen, M, 1040)
+    x = R.rows(xq, xs)
+    for bias in (None, torch.randn(4102, generator=gen).to(dtype).cuda()):
+        outs = fused.forward(xq, xs, bias=bias, epilogue="relu", out_dtype=dtype)
+        at = 0
+        for p, o in zip(parts, outs):
+            n, w = p[0].shape[0], R.matrix(*p)
+            own = None if bias is None else bias[at: at + n].double()
+            z = x @ w.t() if own is None else x @ w.t() + own
+            R.assert_within(o, z.clamp(min=0), R.product_bound(x, w, z, own, dtype), "part")
+            at += n
+
+
+def test_fused_rows_refusals():
+    gen = torch.Generator().manual_seed(4)
+    fused = FusedRows([layer(*R.random_weight(gen, 128, 256)), layer(*R.random_weight(gen, 40, 256))])
+    xq, xs = R.random_rows(gen, 4, 256)
+    with pytest.raises(NQError, match="are needed"):
+        fused.forward(xq)
+    with pytest.raises(NQError, match="codes must be"):
+        fused.forward(torch.zeros((4, 256), device="cuda"), xs)
+    with pytest.raises(NQError, match="output has 159 values, expected 160"):
+        fused.forward(xq, xs, outs=[torch.empty((4, 128), device="cuda"), torch.empty(159, device="cuda")])
+    with pytest.raises(NQError, match="output must be torch.float32"):
+        fused.forward(xq, xs, outs=[torch.empty((4, n), device="cuda", dtype=torch.bfloat16) for n in (128, 40)])
+    with pytest.raises(NQError, match="outputs for a layer of"):
+        fused.forward(xq, xs, outs=[torch.empty((4, 128), device="cuda")])
+    with pytest.raises(NQError, match="bias has 167 values"):
+        fused.forward(xq, xs, bias=torch.zeros(167, device="cuda"))
 
 
 def fused_dequantized(fused, N, K):

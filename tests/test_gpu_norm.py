@@ -84,6 +84,29 @@ def test_constant_rows_and_far_means(D):
     R.assert_within(norm.forward(far), want, e_y, "far mean")
 
 
+@pytest.mark.parametrize("D", [16, 20, 960, 1001])
+def test_huge_constant_rows(D):
+    """Rows of one huge power of two: xh is 0, and what lies behind the row in its block, or behind the last row, adds
+    nothing, although mean x rstd is beyond fp32 there.  (2^116 sums exactly over the rows' powers of two; rstd is 2^20.)"""
+    M = 4097
+    norm = LayerNorm(D, eps=2.0 ** -40)
+    gen = torch.Generator().manual_seed(D)
+    norm.set_params(1 + 0.2 * torch.randn(D, generator=gen), 0.1 * torch.randn(D, generator=gen))
+    x = torch.full((M, D), 2.0 ** 116).cuda()
+    codes, scales, mean, rstd = norm.forward_fp8_train(x)
+    assert torch.equal(mean, x[:, 0]) and (rstd == 2.0 ** 20).all()
+    want = quantize_rows_fp8_block(norm.beta.expand(M, D).contiguous())
+    assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
+    assert torch.equal(norm.forward(x), norm.beta.expand(M, D))
+    gy = torch.ones((M, D)).cuda()
+    gx, dg, db = norm.vjp(x, mean, rstd, gy)
+    assert (db == M).all() and not dg.any()
+    a = norm.gamma.double()
+    # the mean's additions and division, each within half a step of sums of at most sum |a|; the difference; x 2^20 is exact
+    bound = 2.0 ** 20 * R.U * (2 * (D + 1) * a.abs().mean() + (a - a.mean()).abs())
+    R.assert_within(gx, (2.0 ** 20 * (a - a.mean())).expand(M, D), bound.expand(M, D), "gx")
+
+
 @pytest.mark.parametrize("D", [1040, 16400])
 def test_rows_beyond_four_gigabytes(D):
     """The last rows of a call whose rows end beyond 2^32 bytes have the bits of a call of their own."""
@@ -222,12 +245,49 @@ def test_projection_with_a_norm_and_an_adapter():
     R.assert_within(got, base.double() + share, 1.01 * (960 + 8 + 8) * 2 * R.U * mag + R.U * (got.double().abs() + 1e-30), "adapter")
     with pytest.raises(NQError, match="fp32"):
         ad.forward_with(lin, xn, out_dtype=torch.bfloat16)
+    with pytest.raises(NQError, match="differ in shape"):
+        LoRAAdapter(960, 336, 8).forward_with(lin, xn)
     ad.merged = True
+    assert torch.equal(ad.forward_with(lin, xn, out_dtype=torch.bfloat16), lin.forward(xn))
     assert torch.equal(proj_fwd(lin, x, adapter=ad, norm=norm), proj_fwd(lin, x, norm=norm))
 
     q = QLinear(960, 320)
     q.set_weight((torch.randn(320, 960, generator=gen) * 0.05).numpy())
     assert torch.equal(proj_fwd(q, x, norm=norm), q.forward(xn))
+
+
+def test_two_graphs_at_once():
+    """Two recorded backward steps of one norm keep their partial sums apart: replayed together on two streams, each
+    returns the eager bits."""
+    norm, x, gen = inputs(1500, 1024, torch.bfloat16, 5)
+    ins = [(x[:m].clone(), torch.randn(m, 1024, generator=gen).to(torch.bfloat16).cuda()) for m in (1500, 1490)]
+
+    def step(x, gy):
+        y, mean, rstd = norm.forward_train(x)
+        return (y, mean, rstd) + norm.vjp(x, mean, rstd, gy)
+
+    graphs, outs = [], []
+    for a in ins:
+        step(*a)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(*a))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(3):
+        for a in ins:
+            a[0].mul_(0.5), a[1].add_(0.25)
+        want = [step(*a) for a in ins]
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            for got, w in zip(outs[k], want[k]):
+                assert torch.equal(got, w), (turn, k)
 
 
 def test_chain_forward_and_back():
