@@ -75,7 +75,7 @@ struct BlockParams {
     SegTable seg;
 };
 
-// nq_fp8_block_gemm.hip: y = seg.y[0], one part
+// nq_fp8_block_gemm.hip
 bool fp8_block_gemm_applicable(const BlockParams& p);
 double fp8_block_gemm_estimate_us(const BlockParams& p);
 int32_t launch_fp8_block_gemm(const BlockParams& p, hipStream_t s);

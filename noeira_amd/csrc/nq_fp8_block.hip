@@ -366,27 +366,7 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
     for (int t = 0; t < a.seg.nseg; t++) p.vec = p.vec && ((uintptr_t)a.seg.y[t] & line) == 0;
     double tile_us = 0.0;
     const Shape* shape = pick_shape(p, &tile_us);
-    if (fp8_block_gemm_applicable(p)) {
-        // the GEMM writes one part: a row-fused layer's parts run one after the other (they begin on whole blocks)
-        BlockParams part[4];
-        double us = 0.0;
-        for (int t = 0, r0 = 0; t < a.seg.nseg; r0 = a.seg.end[t], t++) {
-            BlockParams& q = part[t] = p;
-            q.w = p.w + (int64_t)(r0 / 16) * p.G * 2048;
-            q.ws = p.ws + (int64_t)(r0 / FP8_BLOCK) * p.G;
-            q.bias = !p.bias ? nullptr : reinterpret_cast<const uint8_t*>(p.bias) + (int64_t)r0 * (p.bias_dtype == NQ_DT_F32 ? 4 : 2);
-            q.N = a.seg.end[t] - r0;
-            q.seg.nseg = 1, q.seg.end[0] = q.N, q.seg.y[0] = a.seg.y[t];
-            us += fp8_block_gemm_estimate_us(q);
-        }
-        if (us < tile_us) {
-            for (int t = 0; t < a.seg.nseg; t++) {
-                const int32_t rc = launch_fp8_block_gemm(part[t], a.stream);
-                if (rc) return rc;
-            }
-            return NQ_OK;
-        }
-    }
+    if (fp8_block_gemm_applicable(p) && fp8_block_gemm_estimate_us(p) < tile_us) return launch_fp8_block_gemm(p, a.stream);
     switch (shape->mt * 8 + shape->nt) {
         case 1 * 8 + 1:
             // K over 16 wavefronts where each keeps two blocks and more: one row's call is bound by the loads under way

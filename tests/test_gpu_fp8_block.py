@@ -299,8 +299,8 @@ def test_fused_rows(M):
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("M", [1100, 2200])
 def test_fused_rows_of_a_batch(M, dtype):
-    """Rows enough that the parts run one after the other on the GEMM (2200; 1100 in one launch of the few-rows kernel,
-    whose sums meet in another order than a part's own): values of the parts, with a bias across all of them."""
+    """Rows enough for the GEMM, whose tiles then lie across the parts' boundaries: values of the parts, with a bias
+    across all of them (the blocks may be added in another order than in a part's own call)."""
     gen = torch.Generator().manual_seed(2)
     parts = [R.random_weight(gen, n, 1040) for n in (2048, 1024, 1030)]
     fused = FusedRows([layer(*p) for p in parts])
