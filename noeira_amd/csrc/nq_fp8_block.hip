@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void
 // in wavefront order (bit-repeatable).  U: blocks requested together.  Both operands go from memory to registers: the
 // weight's tiles are contiguous, every byte of them is read once per 16 MT rows, and at one row nothing else matters.
 // One row over 4096 -> 11008 (45 MB, rotating over copies): 9.1 us in bf16, 4.9 TB/s (a plain copy moves 5.0); 256 rows over
-// 4096 -> 4096: 17.4 - 19, 134 MB from L2 (8.7 TB/s, which bounds every call from about 16 rows on).
+// 4096 -> 4096: 15.2, 134 MB from L2 (11 TB/s, which bounds every call from about 16 rows on).
 template <int MT, int NT, int KW, int U, bool EXACT>
 __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockParams p) {
     constexpr int ROWS = 16 * MT, CH = 16 * NT;
@@ -171,45 +171,59 @@ __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockPara
         wtile[j] = p.w + (int64_t)R * p.G * 2048 + lane * 16;
         wscale[j] = p.ws + (int64_t)(R / 8) * p.G;
     }
-    for (int g0 = wave; g0 < p.G; g0 += KW * U) {
-        i32x4 xv[U][MT][2], wv[U][NT][2];
-        float sx[U][MT], sw[U][NT];
+    static_assert(4 % U == 0, "scales come four blocks at a time");
+    for (int four = wave; four < p.G; four += 4 * KW) {
+        // a row's scales of the next four blocks, one per lane that holds the row: one request for 16 rows instead of four
+        // (16 lines each; as requests of every block's own they were a fifth of those under way)
+        float sx4[MT];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int g = min(g0 + u * KW, p.G - 1);
+        for (int i = 0; i < MT; i++) sx4[i] = p.xs[mrow[i] * p.G + min(four + c * KW, p.G - 1)];
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
+        for (int b = 0; b < 4; b += U) {
+            const int g0 = four + b * KW;
+            if (g0 >= p.G) break;
+            i32x4 xv[U][MT][2], wv[U][NT][2];
+            float sw[U][NT];
 #pragma unroll
-                for (int e = 0; e < 2; e++) wv[u][j][e] = *reinterpret_cast<const i32x4*>(wtile[j] + (int64_t)g * 2048 + e * 1024);
-                sw[u][j] = wscale[j][g];
-            }
+            for (int u = 0; u < U; u++) {
+                const int g = min(g0 + u * KW, p.G - 1);
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
+                for (int j = 0; j < NT; j++) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    // (K is a multiple of 16: a piece lies in the row or behind it, and what lies behind counts as zero)
-                    const int k = 128 * g + 64 * e + 16 * c;
-                    const i32x4 v = *reinterpret_cast<const i32x4*>(p.x + mrow[i] * p.K + (k < p.K ? k : 0));
-                    xv[u][i][e] = k < p.K ? v : i32x4{0, 0, 0, 0};
+                    for (int e = 0; e < 2; e++) wv[u][j][e] = *reinterpret_cast<const i32x4*>(wtile[j] + (int64_t)g * 2048 + e * 1024);
+                    sw[u][j] = wscale[j][g];
                 }
-                sx[u][i] = p.xs[mrow[i] * p.G + g];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (g0 + u * KW < p.G) {
-                Operand<EXACT> w[NT];
-#pragma unroll
-                for (int j = 0; j < NT; j++) w[j] = Operand<EXACT>(wv[u][j][0], wv[u][j][1]);
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const Operand<EXACT> x(xv[u][i][0], xv[u][i][1]);
 #pragma unroll
-                    for (int j = 0; j < NT; j++) {
-                        const f32x4 d = block_sum(w[j], x);
-                        const float s = sx[u][i] * sw[u][j];
+                    for (int e = 0; e < 2; e++) {
+                        // (K is a multiple of 16: a piece lies in the row or behind it, and what lies behind counts as zero)
+                        const int k = 128 * g + 64 * e + 16 * c;
+                        const i32x4 v = *reinterpret_cast<const i32x4*>(p.x + mrow[i] * p.K + (k < p.K ? k : 0));
+                        xv[u][i][e] = k < p.K ? v : i32x4{0, 0, 0, 0};
+                    }
+                }
+            }
 #pragma unroll
-                        for (int t = 0; t < 4; t++) acc[i][j][t] = fmaf(d[t], s, acc[i][j][t]);
+            for (int u = 0; u < U; u++) {
+                float sx[MT];
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+                    sx[i] = __int_as_float(__builtin_amdgcn_ds_bpermute((r + 16 * (b + u)) * 4, __float_as_int(sx4[i])));
+                if (g0 + u * KW < p.G) {
+                    Operand<EXACT> w[NT];
+#pragma unroll
+                    for (int j = 0; j < NT; j++) w[j] = Operand<EXACT>(wv[u][j][0], wv[u][j][1]);
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        const Operand<EXACT> x(xv[u][i][0], xv[u][i][1]);
+#pragma unroll
+                        for (int j = 0; j < NT; j++) {
+                            const f32x4 d = block_sum(w[j], x);
+                            const float s = sx[i] * sw[u][j];
+#pragma unroll
+                            for (int t = 0; t < 4; t++) acc[i][j][t] = fmaf(d[t], s, acc[i][j][t]);
+                        }
                     }
                 }
             }
@@ -279,20 +293,20 @@ int32_t launch_tile(BlockParams p, hipStream_t s) {
 }
 
 // The tile shapes of the few-rows kernel.  A call of it is bound by the operands' way into the CUs: a workgroup brings in
-// 16 (MT + NT) rows of K bytes at about 34 KB per microsecond and CU (8.7 TB/s over the chip, measured at M = 32 .. 512
-// over 4096 x 4096), so of the shapes the one with the lowest estimate is taken; up to two workgroups per CU the fullest CU
-// counts, beyond that the load evens out.  Measured (K = N = 4096, M = 16 / 32 / 64 / 128 / 256, us): 1 x 1 5.5 / 8.5 / 13 / - / -,
-// 1 x 2 6.0 / 7.2 / 11.7 / - / -, 2 x 2 - / 8.7 / 8.8 / 15.0 / -, 2 x 4 - / - / 11.1 / 13.3 / 22.4, 4 x 4 - / - / - / 17 / 17.4.
+// 16 (MT + NT) rows of K bytes at about 55 KB per microsecond and CU, a workgroup after a CU's first adds its meeting in LDS
+// and its stores, and an fp32 y the second half of its products.  Of the shapes the one with the lowest estimate is taken:
+// over 200 calls (1 - 2045 rows, K = 96 .. 11008, N = 17 .. 11008, both y) that and the GEMM's estimate together cost 0.9 %
+// over the best of all shapes of either kernel in the mean, 21 % at worst.  Measured (K = N = 4096, M = 16 / 64 / 128 / 256 in bf16,
+// us): 1 x 1 5.0 / - / - / -, 1 x 2 5.5 / - / - / -, 2 x 2 - / 7.9 / 13.0 / 23, 2 x 4 - / 9.5 / 12.2 / 21, 4 x 4 - / 13.7 / - / 15.2.
 struct Shape {
     int mt, nt;
 };
 constexpr Shape SHAPES[] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}, {4, 4}};
 double tile_estimate_us(const BlockParams& p, const Shape& t) {
-    const double wgs = (double)((p.M - 1) / (16 * t.mt) + 1) * ((p.N - 1) / (16 * t.nt) + 1) / 256.0;
-    const double per_cu = wgs <= 1.0 ? 1.0 : wgs <= 2.0 ? 2.0 : wgs;
-    // (every workgroup after a CU's first adds its meeting in LDS and its stores: 128 k over 8192 x 11008 outputs in tiles of
-    // 4 x 4 took 1.9 us a workgroup)
-    return 2.2 + 0.06 * t.mt * t.nt + per_cu * (double)p.K * 16.0 * (t.mt + t.nt) / 34e3 + (per_cu - 1.0) * 0.1 * t.mt * t.nt;
+    const int64_t wgs = (int64_t)((p.M - 1) / (16 * t.mt) + 1) * ((p.N - 1) / (16 * t.nt) + 1);
+    const double per_cu = (double)((wgs + 255) / 256), tiles = t.mt * t.nt;
+    const double one = (double)p.K * (16.0 * (t.mt + t.nt) / 55e3 + (p.y_dtype == NQ_DT_F32 ? 9e-6 * tiles : 0.0));
+    return 2.9 + 0.10 * tiles + per_cu * one + (per_cu - 1.0) * 0.19 * tiles;
 }
 const Shape* pick_shape(const BlockParams& p, double* us) {
     const Shape* best = nullptr;
@@ -369,22 +383,14 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
     if (fp8_block_gemm_applicable(p) && fp8_block_gemm_estimate_us(p) < tile_us) return launch_fp8_block_gemm(p, a.stream);
     switch (shape->mt * 8 + shape->nt) {
         case 1 * 8 + 1:
-            // K over 16 wavefronts where each keeps two blocks and more: one row's call is bound by the loads under way
-            // (1 row, 4096 -> 11008: 9.1 us against 9.4 - 10 on 8; 11008 -> 4096: 9.0 against 10.1; 16 rows, 4096 -> 4096: 5.7 against 5.4)
-            if (p.G >= 64 || (p.M == 1 && p.G >= 32)) return launch_tile<1, 1, 16, 2>(p, a.stream);
+            // K over 16 wavefronts where each keeps two blocks and more and few rows are read: such a call is bound by the loads
+            // under way (1 row, 4096 -> 11008: 9.5 us against 9.9 on 8; 8 rows, 11008 -> 4096: 10.1 against 11.1; 16: 13.6 against 11.8)
+            if (p.M == 1 ? p.G >= 32 : p.M <= 8 && p.G >= 64) return launch_tile<1, 1, 16, 2>(p, a.stream);
             return launch_tile<1, 1, 8, 2>(p, a.stream);
         case 1 * 8 + 2: return launch_tile<1, 2, 8, 2>(p, a.stream);
         case 2 * 8 + 2: return launch_tile<2, 2, 8, 2>(p, a.stream);
-        // (five to sixteen blocks of K: over 8 wavefronts, one or two each.  135 rows, 960 -> 2567: 5.9 / 6.4 us (bf16 / fp32 y) against
-        // 6.7 / 7.1 on 4; 128 rows, 4096 -> 4096: 13.3 / 16.7 against 13.3 / 13.5)
-        case 2 * 8 + 4:
-            if (p.G > 4 && p.G <= 16) return launch_tile<2, 4, 8, 1>(p, a.stream);
-            return launch_tile<2, 4, 4, 1>(p, a.stream);
-        // (8 wavefronts fill a CU's LDS: only where no CU gets two.  256 rows, 4096 -> 4096 in fp32: 19.6 us against 22.0 on 4; 512 rows:
-        // 37.9 against 33.6)
-        default:
-            if (p.G > 4 && (int64_t)((p.M - 1) / 64 + 1) * ((p.N - 1) / 64 + 1) <= 256) return launch_tile<4, 4, 8, 1>(p, a.stream);
-            return launch_tile<4, 4, 4, 1>(p, a.stream);
+        case 2 * 8 + 4: return launch_tile<2, 4, 8, 1>(p, a.stream);
+        default: return launch_tile<4, 4, 8, 1>(p, a.stream);
     }
 }
 
