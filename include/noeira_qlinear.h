@@ -298,8 +298,8 @@ int32_t nq_layer_norm_fp8_block(const void* x, int32_t x_dtype, const float* gam
  *     gx = rstd * (a - mean_D(a) - xh * mean_D(a * xh)),  dgamma = sum_M gy * xh,  dbeta = sum_M gy
  * gx [M, D] F32 or BF16 (gx may be gy, or x, where the types agree); dgamma, dbeta fp32 [D] are overwritten (zeros for
  * M = 0), or both NULL: no sums over the rows.  Their partial sums lie in `workspace` (16-byte aligned, at least
- * nq_layer_norm_grad_workspace_bytes(M, D)), which holds nothing between calls; two calls that may run at once need
- * one each.  The rows are added in a fixed order: the same inputs give the same bits.  D <= 2^26. */
+ * nq_layer_norm_grad_workspace_bytes(M, D); 0 where a few rows need none), which holds nothing between calls; two calls
+ * that may run at once need one each.  The rows are added in a fixed order: the same inputs give the same bits.  D <= 2^26. */
 int64_t nq_layer_norm_grad_workspace_bytes(int32_t M, int32_t D);
 int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, const float* rstd, const float* gamma,
                            const void* gy, int32_t gy_dtype, void* gx, int32_t gx_dtype, float* dgamma, float* dbeta,

@@ -88,11 +88,15 @@ __device__ __forceinline__ void fetch(Raw<BF16>& r, const void* row, int k, int 
             for (int h = 0; h < (BF16 ? 1 : 2); h++) r.v[h] = p[h];
         }
     } else {
-        uint32_t t[8];
+        // (loads without a branch each, behind which the compiler waits for every one: the row's last value again beyond its end)
+        uint32_t t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (end > 0) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            t[i] = 0;
-            if (k + 16 * i < end) t[i] = BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(row)[k + 16 * i] : reinterpret_cast<const uint32_t*>(row)[k + 16 * i];
+            for (int i = 0; i < 8; i++) {
+                const int at = min(k + 16 * i, end - 1);
+                const uint32_t v = BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(row)[at] : reinterpret_cast<const uint32_t*>(row)[at];
+                t[i] = k + 16 * i < end ? v : 0;
+            }
         }
         if constexpr (BF16) {
             r.v[0] = u32x4{t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16};
@@ -379,6 +383,97 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(const NormGradArg
     }
 }
 
+// Backward in one launch: workgroups of two kinds, which need nothing of each other, since the statistics are given.  The first
+// `columns` take 16 columns each, one value per thread and row, their rows dealt over THREADS / 16 slices whose sums meet in
+// LDS in order: dgamma and dbeta, no partials.  The others are teams of T threads, a row each: gx.  x and gy are read twice,
+// the second time from L2.
+template <int T, int NV, int THREADS, bool XB, bool GB, bool VEC>
+__global__ __launch_bounds__(THREADS) void layer_norm_grad_once_kernel(const NormGradArgs a, int32_t columns, int32_t rounds) {
+    constexpr int PER = THREADS / T, SLICES = THREADS / 16;
+    __shared__ float lds[2][PER][2][T / 64];
+    __shared__ float meet[2][SLICES][16];
+    if ((int)blockIdx.x < columns) {
+        const int c = threadIdx.x % 16, s = threadIdx.x / 16;
+        const int64_t d = (int64_t)blockIdx.x * 16 + c;
+        float g = 0.0f, b = 0.0f;
+        if (d < a.D) {
+#pragma unroll 8
+            for (int64_t m = s; m < a.M; m += SLICES) {
+                const float t = load1(a.gy, GB ? NQ_DT_BF16 : NQ_DT_F32, m * a.D + d);
+                g += t * ((load1(a.x, XB ? NQ_DT_BF16 : NQ_DT_F32, m * a.D + d) - a.mean[m]) * a.rstd[m]);
+                b += t;
+            }
+        }
+        meet[0][s][c] = g, meet[1][s][c] = b;
+        __syncthreads();
+        if (s < 2 && d < a.D) {
+            float v = 0.0f;
+#pragma unroll 8
+            for (int q = 0; q < SLICES; q++) v += meet[s][q][c];
+            (s == 0 ? a.dgamma : a.dbeta)[d] = v;
+        }
+        return;
+    }
+    const int t = threadIdx.x % T, mine = (int)threadIdx.x / T, wave = t / 64;
+    const int64_t teams = (int64_t)((int)gridDim.x - columns) * PER;
+    const float inv_d = 1.0f / (float)a.D;
+    const uint8_t* x = reinterpret_cast<const uint8_t*>(a.x);
+    const uint8_t* gy = reinterpret_cast<const uint8_t*>(a.gy);
+    constexpr int xs = XB ? 2 : 4, gs = GB ? 2 : 4;
+    float w[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        Raw<false> r;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[v][i] = 1.0f;
+        if (a.gamma) fetch<false, VEC>(r, a.gamma, first_index<T, VEC>(t, v), a.D), widen<false>(r, w[v]);
+    }
+    int64_t m = (int64_t)((int)blockIdx.x - columns) * PER + mine;
+    for (int32_t k = 0; k < rounds; k++, m += teams) {
+        const int end = m < a.M ? a.D : 0;  // (a team without a row left takes part in the barriers with zeros)
+        Raw<XB> rx[NV];
+        Raw<GB> rg[NV];
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            fetch<XB, VEC>(rx[v], x + m * a.D * xs, first_index<T, VEC>(t, v), end);
+            fetch<GB, VEC>(rg[v], gy + m * a.D * gs, first_index<T, VEC>(t, v), end);
+        }
+        const float mean = end > 0 ? a.mean[m] : 0.0f, rstd = end > 0 ? a.rstd[m] : 0.0f;
+        float xh[NV][8], f[NV][8];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            widen<XB>(rx[v], xh[v]);
+            widen<GB>(rg[v], f[v]);
+            const int at = first_index<T, VEC>(t, v);
+            const float rv = !VEC || at < a.D ? rstd : 0.0f;  // (behind the row: as in the kernel above)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                xh[v][i] = VEC || at + 16 * i < a.D ? (xh[v][i] - mean) * rv : 0.0f;
+                f[v][i] *= w[v][i];
+                s1 += f[v][i];
+                s2 += f[v][i] * xh[v][i];
+            }
+        }
+        float c1 = wave_sum(s1), c2 = wave_sum(s2);
+        if constexpr (T > 64) {
+            float(&at)[2][T / 64] = lds[k & 1][mine];
+            if ((threadIdx.x & 63) == 0) at[0][wave] = c1, at[1][wave] = c2;
+            __syncthreads();
+            c1 = at[0][0], c2 = at[1][0];
+#pragma unroll
+            for (int q = 1; q < T / 64; q++) c1 += at[0][q], c2 += at[1][q];
+        }
+        c1 *= inv_d, c2 *= inv_d;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[v][i] = rstd * (f[v][i] - c1 - xh[v][i] * c2);
+            put<VEC>(a.gx, a.gx_dtype, m * a.D, first_index<T, VEC>(t, v), end, f[v]);
+        }
+    }
+}
+
 // rows beyond 16384 values: gx, one workgroup per row, two passes
 __global__ __launch_bounds__(1024) void layer_norm_grad_x_long_kernel(const NormGradArgs a) {
     __shared__ float lds[2][16];
@@ -445,7 +540,7 @@ __global__ __launch_bounds__(256) void zero_kernel(float* p, float* q, int32_t n
 
 constexpr int MAX_HELD = 16384;
 
-// threads per row and vectors per thread: backward
+// threads per row and vectors per thread: backward with partials
 void grad_team_of(int32_t D, int* T, int* NV) {
     *T = D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024;
     *NV = D <= *T * 8 ? 1 : 2;
@@ -474,8 +569,18 @@ int32_t launch_norm(const NormArgs& a, hipStream_t s) {
     return NQ_OK;
 }
 
-// partials of a call: one workgroup per CU, fewer where the rows run out
-int32_t partials_of(int32_t M, int32_t D) {
+// Where both gradients come from one launch and no partials (layer_norm_grad_once_kernel): its columns take a time that grows
+// with M / slices, and the rows are read twice.  Partials / one launch, us: 1 x 960 7.4 / 4.4 (a launch saved), 333 x 1001 fp32
+// 9.0 / 4.4, 1024 x 960 fp32 9.9 / 7.3, 2048 x 960 12.9 / 12.2, 512 x 4096 fp32 18.4 / 10.0, 1024 x 4096 fp32 20.6 / 18.3, 1536 x 4096
+// 25.7 / 27.4, 1024 x 8192 47.8 / 36.7, 1024 x 11008 51.9 / 54.4; rows of odd length, whose columns lie across lines: 512 x
+// 4095 15.6 / 12.0, 1024 x 4095 18.5 / 23.2, 333 x 8191 17.1 / 18.2, but 512 x 11007 39.4 / 36.2 (the other kernel's 16 values per
+// thread spill there).
+bool grad_once(int32_t M, int32_t D) {
+    return D <= MAX_HELD && M <= 1024 && (int64_t)M * D <= (D % 8 == 0 || D > 8192 ? 1 << 23 : 1 << 21);
+}
+
+// workgroups of the other kernels, one per CU, fewer where the rows run out: as many partials
+int32_t grad_workgroups(int32_t M, int32_t D) {
     if (D > MAX_HELD) return (int32_t)std::min<int64_t>(64, ((int64_t)M + 63) / 64);
     int T, NV;
     grad_team_of(D, &T, &NV);
@@ -521,6 +626,36 @@ int32_t launch_grad_held(const NormGradArgs& a, int32_t P, hipStream_t s) {
     }
 }
 
+template <int T, int NV, int THREADS>
+int32_t launch_once(const NormGradArgs& a, bool columns, bool rows, hipStream_t s) {
+    constexpr int64_t PER = THREADS / T;
+    const int32_t nc = columns ? (a.D - 1) / 16 + 1 : 0;
+    const int32_t nr = rows ? (int32_t)std::min<int64_t>((a.M + PER - 1) / PER, 256 * (2048 / THREADS)) : 0;
+    const int32_t rounds = rows ? (int32_t)((a.M + nr * PER - 1) / (nr * PER)) : 0;
+    const bool xb = a.x_dtype == NQ_DT_BF16, gb = a.gy_dtype == NQ_DT_BF16, vec = a.D % 8 == 0;
+#define NQ_GO(X, G, V) \
+    hipLaunchKernelGGL((layer_norm_grad_once_kernel<T, NV, THREADS, X, G, V>), dim3(nc + nr), dim3(THREADS), 0, s, a, nc, rounds)
+#define NQ_GV(X, G)             \
+    if (vec) NQ_GO(X, G, true); \
+    else NQ_GO(X, G, false)
+    if (xb && gb) { NQ_GV(true, true); }
+    else if (xb) { NQ_GV(true, false); }
+    else if (gb) { NQ_GV(false, true); }
+    else { NQ_GV(false, false); }
+#undef NQ_GV
+#undef NQ_GO
+    NQ_HIP(hipGetLastError());
+    return NQ_OK;
+}
+
+int32_t launch_grad_once(const NormGradArgs& a, bool columns, bool rows, hipStream_t s) {
+    if (a.D <= 512) return launch_once<64, 1, 1024>(a, columns, rows, s);
+    if (a.D <= 2048) return launch_once<256, 1, 512>(a, columns, rows, s);
+    if (a.D <= 4096) return launch_once<512, 1, 512>(a, columns, rows, s);
+    if (a.D <= 8192) return launch_once<1024, 1, 1024>(a, columns, rows, s);
+    return launch_once<1024, 2, 1024>(a, columns, rows, s);
+}
+
 }  // namespace
 
 int32_t launch_layer_norm(const NormArgs& a, hipStream_t s) {
@@ -541,7 +676,7 @@ int32_t launch_layer_norm(const NormArgs& a, hipStream_t s) {
     }
 }
 
-int64_t layer_norm_grad_partial_bytes(int32_t M, int32_t D) { return (int64_t)partials_of(M, D) * 2 * D * 4; }
+int64_t layer_norm_grad_partial_bytes(int32_t M, int32_t D) { return grad_once(M, D) ? 0 : (int64_t)grad_workgroups(M, D) * 2 * D * 4; }
 
 int32_t launch_layer_norm_grad(const NormGradArgs& a, hipStream_t s) {
     if (a.M == 0) {
@@ -550,7 +685,16 @@ int32_t launch_layer_norm_grad(const NormGradArgs& a, hipStream_t s) {
         NQ_HIP(hipGetLastError());
         return NQ_OK;
     }
-    const int32_t P = partials_of(a.M, a.D);
+    if (grad_once(a.M, a.D)) {
+        // (gx written over what the columns read: they go first, in a launch of their own; gx has the same bits either way)
+        const bool over = a.gx == a.x || a.gx == a.gy;
+        if (a.dgamma && over) {
+            const int32_t rc = launch_grad_once(a, true, false, s);
+            if (rc) return rc;
+        }
+        return launch_grad_once(a, a.dgamma && !over, true, s);
+    }
+    const int32_t P = grad_workgroups(a.M, a.D);
     if (a.D > MAX_HELD) {
         if (a.dgamma) {  // (the columns first: gx may be gy's own memory)
             hipLaunchKernelGGL(layer_norm_grad_w_long_kernel, dim3((unsigned)((a.D - 1) / 64 + 1), (unsigned)P), dim3(64), 0, s, a);

@@ -146,7 +146,8 @@ def test_non_finite_rows_stay_alone():
 
 @pytest.mark.parametrize("gdtype", DTYPES, ids=["gy f32", "gy bf16"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
-@pytest.mark.parametrize("M,D", SHAPES)
+@pytest.mark.parametrize("M,D", SHAPES + [(1024, 65), (1025, 64), (4200, 129), (1900, 960), (700, 4095), (90, 8191), (300, 8191),
+                                         (1100, 8192), (70, 11007), (800, 11007), (65, 16384)])
 def test_gradients(M, D, dtype, gdtype):
     norm, x, gen = inputs(M, D, dtype, 1)
     gy = torch.randn(M, D, generator=gen).to(gdtype).cuda()
