@@ -120,9 +120,10 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int32_t k = (int32_t)g * 128 + 16 * i + l;
-                v[i] = k >= K ? 0.0f
-                              : BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(x)[base + k] << 16)
-                                     : reinterpret_cast<const float*>(x)[base + k];
+                const int64_t at = base + min(k, K - 1);  // (no branch per load, behind which each would be waited for)
+                const float w = BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(x)[at] << 16)
+                                     : reinterpret_cast<const float*>(x)[at];
+                v[i] = k < K ? w : 0.0f;
             }
             const uint2 q = quantize_block16(v, s);
 #pragma unroll
@@ -352,8 +353,8 @@ int32_t launch_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* 
     if (blocks > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: more than 2^31 - 1 blocks of 128");
     const bool bf16 = x_dtype == NQ_DT_BF16, vec = K % 8 == 0;
 #define NQ_QB(B, V)                                                                                                        \
-    hipLaunchKernelGGL((quantize_rows_fp8_block_kernel<B, V>), dim3((unsigned)std::min<int64_t>((blocks + 15) / 16, (1 << 24) - 1)), dim3(256), 0, s, x, \
-                       codes, scales, K, (uint32_t)G, (uint32_t)blocks)
+    hipLaunchKernelGGL((quantize_rows_fp8_block_kernel<B, V>), dim3((unsigned)std::min<int64_t>((blocks + 15) / 16, (1 << 24) - 1)), \
+                       dim3(256), 0, s, x, codes, scales, K, (uint32_t)G, (uint32_t)blocks)
     if (bf16 && vec) NQ_QB(true, true);
     else if (bf16) NQ_QB(true, false);
     else if (vec) NQ_QB(false, true);
