@@ -19,15 +19,19 @@
 // SIMD.  On 128 x 128 tiles LDS is the bound outright (128 KiB per 512 cycles of products: 0.47 us a stage; 18.2 - 20.6 us
 // a round at K = 4096).  With an fp32 y the two bf16 products per fp8 one and 16 conversions per fragment take 239 us
 // (1.15 PFLOP/s; a library bf16 product of the same size 232).
+#include <algorithm>
+
 #include "nq_fp8_block.h"
 
 namespace nq {
 
 namespace {
 
-template <int BM, int BN, int WM, int WN, int NB, bool EXACT>
+// KS = 2: two groups of WM x WN wavefronts, each with stage buffers of its own, take the blocks of K in turn, and the second
+// one's results are added to the first one's through LDS at the end.
+template <int BM, int BN, int WM, int WN, int NB, int KS, bool EXACT>
 __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
-    constexpr int WAVES = WM * WN;
+    constexpr int WAVES = WM * WN;  // of a group
     constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
     constexpr int PAIRS = TJ / 2;
     constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB;  // bytes of a stage
@@ -36,11 +40,14 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     constexpr int CHUNK_BYTES = BM * 16 + 256;                    // scales of four stages: [BM][4], then [BN / 128][4]
     static_assert(TJ % 2 == 0 && PAIRS % 2 == 0 && BN / WN <= 128 && SW < WAVES && BM % (8 * WAVES) == 0 && BN % (16 * WAVES) == 0, "tile");
     static_assert(NB >= 2 && NB <= 4 && (NB > 2 || PAIRS >= 3), "the places of the transfers; three buffers of scales");
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    typedef __attribute__((address_space(3))) void lptr_t;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t*)lds;
+    constexpr int GROUP = NB * STAGE + 3 * CHUNK_BYTES;  // LDS of a group
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_all[];
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = KS == 1 ? 0 : wave_all / WAVES, wave = KS == 1 ? wave_all : wave_all % WAVES;
+    uint8_t* const lds = lds_all + group * GROUP;
+    typedef __attribute__((address_space(3))) void lptr_t;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t*)lds_all + group * GROUP;
     const int wm = wave / WN, wn = wave % WN;
 
     // ---- tile: ids are dealt round-robin to the 8 XCDs, so each XCD is given one contiguous run, and runs walk bands of 8
@@ -81,7 +88,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     uint32_t ibuf = scales0 + CHUNK_BYTES;  // ... and the buffer it goes to
     auto scale_dma = [&](int quarter, int from, uint32_t buffer) {
         const int row = sx_wave ? (quarter * SW + wave) * 16 + lane / 4 : lane / 4;
-        const uint32_t o = ((uint32_t)min(row, srow_end - 1) * (uint32_t)p.G + (uint32_t)min(from + lane % 4, p.G - 1)) * 4;
+        const uint32_t o = ((uint32_t)min(row, srow_end - 1) * (uint32_t)p.G + (uint32_t)min((from + lane % 4) * KS + group, p.G - 1)) * 4;
         const uint32_t m0v = lds0 + buffer + (sx_wave ? (uint32_t)(quarter * SW + wave) * 256 : BM * 16);
         const float* s = sbase;
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
@@ -94,25 +101,26 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     // 16 behind K exists in the first tile's last block, its very last)
     const bool ragged = p.K % 128 != 0;
     const uint8_t* const zeros = p.w + (int64_t)(p.G - 1) * 2048 + 1024 + 48 * 16;
-    const int KT = p.G;
+    const int KT = (p.G - 1) / KS + 1;  // (in the last stage of an odd number of blocks the second group repeats the last, times 0)
     // transfer t of stage st into the buffer at LDS address `at`
     auto dma = [&](auto tc, auto fullc, int st, uint32_t at) {
         constexpr int t = decltype(tc)::value;
-        constexpr bool FULL = decltype(fullc)::value;  // the stage is known to be a whole block of K
+        constexpr bool FULL = decltype(fullc)::value;  // the stage is known to be whole blocks of K
+        const int blk = FULL ? st * KS + group : min(st * KS + group, p.G - 1);
         if constexpr (t < DX) {
             const uint32_t m0v = at + (uint32_t)(wave * DX + t) * 1024;
-            if (!FULL && ragged && st == KT - 1) {
-                const uint8_t* a = st * 128 + xk[t] < p.K ? xbase + xoff[t] + (int64_t)st * 128 : zeros;
+            if (!FULL && ragged && blk == p.G - 1) {
+                const uint8_t* a = blk * 128 + xk[t] < p.K ? xbase + xoff[t] + (int64_t)blk * 128 : zeros;
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0v), "v"(a) : "memory");
             } else {
-                const uint8_t* s = xbase + (int64_t)st * 128;
+                const uint8_t* s = xbase + (int64_t)blk * 128;
                 const uint32_t o = xoff[t];
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
             }
         } else {
             constexpr int u = t - DX;
             const uint32_t m0v = at + XB + (uint32_t)(wave * DW + u) * 1024;
-            const uint8_t* s = wtile[u / 2] + (int64_t)st * 2048 + (u & 1) * 1024;
+            const uint8_t* s = wtile[u / 2] + (int64_t)blk * 2048 + (u & 1) * 1024;
             const uint32_t o = woff;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0v), "v"(o), "s"(s) : "memory");
         }
@@ -241,7 +249,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             constexpr bool END = pr == PAIRS - 1;
             if constexpr (pr == 0) {
 #pragma unroll
-                for (int i = 0; i < TI; i++) s[i] = sx[i] * sw;
+                for (int i = 0; i < TI; i++) s[i] = KS > 1 && LAST && st * KS + group >= p.G ? 0.0f : sx[i] * sw;
             }
             if constexpr (NB == 2 && pr == 1 && !LAST) {
                 if (more) {
@@ -323,7 +331,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
             prev = at, at = next;
         }
     };
-    walk(integral_constant<int, 0>{}, (ragged ? KT - 1 : KT) - AHEAD);
+    walk(integral_constant<int, 0>{}, (ragged ? p.G - 1 : p.G) / KS - AHEAD);
     walk(integral_constant<int, 1>{}, KT - 1);
     stage(integral_constant<int, 2>{}, KT - 1, at, 0, 0);
     settle_into(Q - 2, late[0], late_s);
@@ -342,6 +350,18 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                                                     : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[n] << 16);
         }
     __syncthreads();  // (nothing is under way: the last requests were waited for a stage ago)
+    if constexpr (KS == 2) {
+        static_assert(WAVES * TI * TJ * 1024 <= GROUP, "the second group's results in its own LDS");
+        f32x4* const meet = reinterpret_cast<f32x4*>(lds_all + GROUP) + wave * TI * TJ * 64 + lane;
+        if (group == 1) {
+#pragma unroll
+            for (int q = 0; q < TI * TJ; q++) meet[q * 64] = acc[q / TJ][q % TJ];
+        }
+        __syncthreads();
+        if (group == 1) return;
+#pragma unroll
+        for (int q = 0; q < TI * TJ; q++) acc[q / TJ][q % TJ] += meet[q * 64];
+    }
 
     // ---- epilogue: a lane holds token 16 i + r and channels 16 j + 4 c .. + 3.  A wavefront stages 32 tokens at a time in
     // LDS of its own and writes them as 128-bit stores, whole rows of its channels.
@@ -390,7 +410,7 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
         } else if (width > col) {
             // rows that do not begin on 16 bytes, or end inside the tile: 4 bytes per lane, adjacent lanes adjacent (bf16 rows
             // that begin on an odd element: pairs from the second one on, and the ends alone).  Every row's loads and stores without
-            // a branch: 4145 rows over 368 -> 6739 in bf16 41.1 us, with one loop per row 46.0
+            // a branch: 1024 rows over 960 -> 2567 in bf16 10.2 us, with a loop of its own per row 14.6, 2560 channels 9.0
             const int limit = min(CH, width - col);
             if constexpr (EXACT) {
                 static_assert(CH == 64, "a row per instruction");
@@ -402,23 +422,22 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
                 }
             } else {
                 constexpr int LPR = CH / 2, RPI = 64 / LPR;
-                const int j = lane % LPR;
+                const int j = lane % LPR, m = wm0 + 16 * ip + lane / LPR;
+                uint16_t* const d = reinterpret_cast<uint16_t*>(y) + (int64_t)m * width + col;
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(stg + lane / LPR * ROWB) + j;
 #pragma unroll 8
                 for (int t = 0; t < 32 / RPI; t++) {
-                    const int row = t * RPI + lane / LPR, m = wm0 + 16 * ip + row;
-                    const int64_t first = (int64_t)m * width + col;
-                    const uint32_t* src = reinterpret_cast<const uint32_t*>(stg + row * ROWB);
-                    const uint32_t w0 = src[j], w1 = src[j + 1];  // (a staged row is followed by 16 spare bytes)
-                    const bool odd = ((uintptr_t)y / 2 + first) & 1;
-                    const uint32_t pair = odd ? w0 >> 16 | w1 << 16 : w0;
-                    uint16_t* d = reinterpret_cast<uint16_t*>(y) + first;
-                    const int e = 2 * j + odd, end = m < p.M ? limit : 0;
-                    if (e + 1 < end)
-                        *reinterpret_cast<uint32_t*>(d + e) = pair;
-                    else if (e < end)
-                        d[e] = (uint16_t)pair;
-                    if (odd && j == 0 && end > 0) d[0] = (uint16_t)w0;
+                    const uint32_t w0 = src[t * RPI * ROWB / 4], w1 = src[t * RPI * ROWB / 4 + 1];  // (16 spare bytes behind a row)
+                    const int odd = (int)((uintptr_t)d / 2 + t * RPI * width) & 1, e = 2 * j + odd;
+                    if (m + t * RPI < p.M && e + 1 < limit)
+                        *reinterpret_cast<uint32_t*>(d + (int64_t)t * RPI * width + e) = odd ? w0 >> 16 | w1 << 16 : w0;
                 }
+                // the ends alone: lanes 2 r and 2 r + 1 look after row r's first and last element
+                const int r1 = lane / 2, end = lane & 1 ? limit - 1 : 0;
+                uint16_t* const d1 = reinterpret_cast<uint16_t*>(y) + (int64_t)(wm0 + 16 * ip + r1) * width + col;
+                const int odd1 = (int)((uintptr_t)d1 / 2) & 1;
+                if (wm0 + 16 * ip + r1 < p.M && (lane & 1 ? (limit - odd1) & 1 : odd1))
+                    d1[end] = reinterpret_cast<const uint16_t*>(stg + r1 * ROWB)[end];
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -427,24 +446,24 @@ __device__ __forceinline__ void block_gemm_body(const BlockParams& p) {
     }
 }
 
-template <int BM, int BN, int NB>
-constexpr size_t lds_bytes() { return (size_t)NB * (BM + BN) * 128 + 3 * (BM * 16 + 256); }
+template <int BM, int BN, int NB, int KS>
+constexpr size_t lds_bytes() { return KS * ((size_t)NB * (BM + BN) * 128 + 3 * (BM * 16 + 256)); }
 
-template <int BM, int BN, int WM, int WN, int NB, bool EXACT>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_block_gemm_kernel(const BlockParams p) {
-    block_gemm_body<BM, BN, WM, WN, NB, EXACT>(p);
+template <int BM, int BN, int WM, int WN, int NB, int KS, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN * KS) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_block_gemm_kernel(const BlockParams p) {
+    block_gemm_body<BM, BN, WM, WN, NB, KS, EXACT>(p);
 }
 
 // `grid`: the first that many tiles of the order only (0: all of the region from m_base, n_base on)
-template <int BM, int BN, int WM, int WN, int NB, bool EXACT>
+template <int BM, int BN, int WM, int WN, int NB, int KS, bool EXACT>
 int32_t launch(BlockParams p, hipStream_t s, int64_t grid = 0) {
     static LdsAttrOnce attr;
     p.tiles_m = (p.M - p.m_base - 1) / BM + 1, p.tiles_n = (p.N - p.n_base - 1) / BN + 1;
     if (grid == 0) grid = (int64_t)p.tiles_m * p.tiles_n;
     if (grid * 512 > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
-    const void* kernel = reinterpret_cast<const void*>(&fp8_block_gemm_kernel<BM, BN, WM, WN, NB, EXACT>);
-    NQ_HIP(set_max_lds_once(attr, kernel, lds_bytes<BM, BN, NB>()));
-    hipLaunchKernelGGL((fp8_block_gemm_kernel<BM, BN, WM, WN, NB, EXACT>), dim3((unsigned)grid), dim3(64 * WM * WN), (lds_bytes<BM, BN, NB>()), s, p);
+    const void* kernel = reinterpret_cast<const void*>(&fp8_block_gemm_kernel<BM, BN, WM, WN, NB, KS, EXACT>);
+    NQ_HIP(set_max_lds_once(attr, kernel, lds_bytes<BM, BN, NB, KS>()));
+    hipLaunchKernelGGL((fp8_block_gemm_kernel<BM, BN, WM, WN, NB, KS, EXACT>), dim3((unsigned)grid), dim3(64 * WM * WN * KS), (lds_bytes<BM, BN, NB, KS>()), s, p);
     NQ_HIP(hipGetLastError());
     return NQ_OK;
 }
@@ -454,24 +473,31 @@ int32_t launch(BlockParams p, hipStream_t s, int64_t grid = 0) {
 // Measured over M = 256 .. 8192, K = 960 and 4096, N = 960 .. 11008 (K = 4096, N = 4096; M = 256 / 512 / 1024 / 2048 / 4096):
 //   bf16 y   128 x 128: 18.2 / 18.5 / 20.6 / 44.6 / 89     128 x 256: 26.7 / 27.0 / 27.7 / 35.8 / 71
 //            256 x 256: 46.5 / 46.8 / 47.1 / 50.1 / 60.4
+//             64 x 128, K dealt over two groups: 15.3 / 16.0 / 29.5 / - / -
 //   fp32 y    64 x 128: 26.0 / 26.6 / 39.6 / 77 / 153      128 x 128: 33.7 / 34.5 / 36.8 / 72 / 141
-//            256 x 128: 54.1 / 54.8 / 56.6 / 61.5 / 120
+//            256 x 128: 54.1 / 54.8 / 56.6 / 61.5 / 120     64 x 128, two groups: 20.9 / 22.2 / 40.5 / - / -
+// (Two groups of four wavefronts: alone on its SIMD a wavefront's multiply-adds stand in the way of its products; two share it,
+// each with a block of its own.  Only 64 x 128 tiles leave room in LDS for two groups' three buffers.)
 struct Form {
     int bm, bn;
     double fixed, step, crowd;
     int from, full;
 };
 constexpr Form F256{256, 256, 8.0, 1.20, 0.40, 64, 256}, F128x256{128, 256, 5.8, 0.665, 0.275, 128, 256},
-    F128{128, 128, 4.5, 0.44, 0.06, 128, 256}, E256x128{256, 128, 6.5, 1.52, 0.20, 64, 256},
-    E128{128, 128, 4.5, 0.92, 0.09, 128, 256}, E64{64, 128, 4.5, 0.69, 0.41, 256, 512};
+    F128{128, 128, 4.5, 0.44, 0.06, 128, 256}, F64K2{64, 128, 4.2, 0.36, 0.02, 128, 256},
+    E256x128{256, 128, 6.5, 1.52, 0.20, 64, 256}, E128{128, 128, 4.5, 0.92, 0.09, 128, 256},
+    E64{64, 128, 4.5, 0.69, 0.41, 256, 512}, E64K2{64, 128, 5.5, 0.485, 0.04, 128, 256};
 
-double estimate(const Form& f, int64_t workgroups, int G) {
+// `off`: what rows off 16 bytes cost per 64 x 32 results of a wavefront (the last stores of the kernel: 1.2 us in bf16, 0.5 in fp32)
+double estimate(const Form& f, int64_t workgroups, int G, double off) {
     const int64_t rounds = (workgroups + f.full - 1) / f.full;
     const double in_round = (double)workgroups / (double)rounds;
     const double crowd = in_round > f.from ? (in_round - f.from) / (double)(f.full - f.from) : 0.0;
-    return (double)rounds * (f.fixed + G * (f.step + f.crowd * crowd));
+    return (double)rounds * (f.fixed + off * std::max(1, f.bm * f.bn / 16384) + G * (f.step + f.crowd * crowd));
 }
-double estimate(const Form& f, int M, int N, int G) { return estimate(f, (int64_t)((M - 1) / f.bm + 1) * ((N - 1) / f.bn + 1), G); }
+double estimate(const Form& f, int M, int N, int G, double off) {
+    return estimate(f, (int64_t)((M - 1) / f.bm + 1) * ((N - 1) / f.bn + 1), G, off);
+}
 
 // The 256 x 256 tiles that do not fill a round of 256 workgroups go on 128 x 256 tiles in a second launch, where they are
 // at most half a round and whole columns of the last band of 8 row tiles (M = 8192, N = 11008: 96 of 1376, 12 columns).
@@ -480,20 +506,25 @@ int64_t leftover(int M, int N) {
     const int64_t tm = (M - 1) / 256 + 1, tn = (N - 1) / 256 + 1, rest = tm * tn % 256, rows = tm - (tm - 1) / 8 * 8;
     return tm * tn > 256 && rest > 0 && rest <= 128 && rest % rows == 0 && rest / rows <= tn ? rest : 0;
 }
-double estimate256(int M, int N, int G) {
+double estimate256(int M, int N, int G, double off) {
     const int64_t tiles = (int64_t)((M - 1) / 256 + 1) * ((N - 1) / 256 + 1), rest = leftover(M, N);
-    return rest ? estimate(F256, tiles - rest, G) + estimate(F128x256, 2 * rest, G) : estimate(F256, tiles, G);
+    return rest ? estimate(F256, tiles - rest, G, off) + estimate(F128x256, 2 * rest, G, off) : estimate(F256, tiles, G, off);
 }
 
 // the form of lowest estimate and that estimate
 const Form* pick(const BlockParams& p, double* us) {
     const bool exact = p.y_dtype == NQ_DT_F32;
+    const double off = p.N % (exact ? 4 : 8) == 0 ? 0.0 : exact ? 0.5 : 1.2;
     const Form* best = exact ? &E256x128 : &F256;
-    *us = exact ? estimate(E256x128, p.M, p.N, p.G) : estimate256(p.M, p.N, p.G);
-    for (const Form* f : {exact ? &E128 : &F128x256, exact ? &E64 : &F128}) {
-        const double t = estimate(*f, p.M, p.N, p.G);
-        if (t < *us) *us = t, best = f;
-    }
+    *us = exact ? estimate(E256x128, p.M, p.N, p.G, off) : estimate256(p.M, p.N, p.G, off);
+    const auto consider = [&](const Form& f) {
+        const double t = estimate(f, p.M, p.N, p.G, off);
+        if (t < *us) *us = t, best = &f;
+    };
+    if (exact)
+        consider(E128), consider(E64), consider(E64K2);
+    else
+        consider(F128x256), consider(F128), consider(F64K2);
     return best;
 }
 
@@ -513,19 +544,21 @@ double fp8_block_gemm_estimate_us(const BlockParams& p) {
 int32_t launch_fp8_block_gemm(const BlockParams& p, hipStream_t s) {
     double us;
     const Form* f = pick(p, &us);
-    if (f == &E64) return launch<64, 128, 2, 2, 3, true>(p, s);
-    if (f == &E128) return launch<128, 128, 4, 2, 4, true>(p, s);
-    if (f == &E256x128) return launch<256, 128, 4, 2, 3, true>(p, s);
-    if (f == &F128) return launch<128, 128, 4, 2, 4, false>(p, s);
-    if (f == &F128x256) return launch<128, 256, 4, 2, 3, false>(p, s);
+    if (f == &E64) return launch<64, 128, 2, 2, 3, 1, true>(p, s);
+    if (f == &E64K2) return launch<64, 128, 2, 2, 3, 2, true>(p, s);
+    if (f == &E128) return launch<128, 128, 4, 2, 4, 1, true>(p, s);
+    if (f == &E256x128) return launch<256, 128, 4, 2, 3, 1, true>(p, s);
+    if (f == &F64K2) return launch<64, 128, 2, 2, 3, 2, false>(p, s);
+    if (f == &F128) return launch<128, 128, 4, 2, 4, 1, false>(p, s);
+    if (f == &F128x256) return launch<128, 256, 4, 2, 3, 1, false>(p, s);
     const int64_t rest = leftover(p.M, p.N);
-    if (!rest) return launch<256, 256, 4, 2, 2, false>(p, s);
+    if (!rest) return launch<256, 256, 4, 2, 2, 1, false>(p, s);
     const int tm = (p.M - 1) / 256 + 1, tn = (p.N - 1) / 256 + 1, rows = tm - (tm - 1) / 8 * 8;
-    const int32_t rc = launch<256, 256, 4, 2, 2, false>(p, s, (int64_t)tm * tn - rest);
+    const int32_t rc = launch<256, 256, 4, 2, 2, 1, false>(p, s, (int64_t)tm * tn - rest);
     if (rc) return rc;
     BlockParams q = p;
     q.m_base = (tm - rows) * 256, q.n_base = (tn - (int)(rest / rows)) * 256;
-    return launch<128, 256, 4, 2, 3, false>(q, s);
+    return launch<128, 256, 4, 2, 3, 1, false>(q, s);
 }
 
 }  // namespace nq

@@ -114,7 +114,10 @@ SHAPES = [(1, 16, 1), (1, 128, 16), (1, 960, 2560), (1, 4096, 1040), (2, 272, 12
           # a hundred tiles of 256 x 256 and more: one block of K, part of one, two, an odd and an even number of them
           (2100, 128, 4100), (3000, 16, 2832), (2049, 256, 4104), (2304, 656, 4001), (4096, 1024, 2048),
           # the other tiles of the GEMM, and tiles left over after the last full round
-          (500, 496, 4001), (1000, 512, 4000), (2045, 528, 4090), (4093, 272, 4345)]
+          (500, 496, 4001), (1000, 512, 4000), (2045, 528, 4090), (4093, 272, 4345),
+          # the blocks of K dealt over two groups of wavefronts: one block, an odd and an even number, part of a last one
+          (220, 16, 5000), (313, 128, 4001), (190, 256, 3000), (282, 272, 5000), (282, 400, 5000), (500, 1408, 3001), (700, 1040, 2050),
+          (4000, 784, 500), (512, 3200, 2100)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
@@ -230,6 +233,32 @@ def test_infinite_scales_follow_ieee():
     got = layer(wq, torch.ones((1, 2), device="cuda")).forward_a8(xq, xs, out_dtype=torch.float32)
     assert got[0, 0] == 256 and got[0, 1] == -256 and got[0, 2] == 0
     assert got[1, 0] == float("inf") and got[1, 1] == -float("inf") and torch.isnan(got[1, 2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(220, 384, 3000), (500, 1408, 3001), (700, 1040, 2050)])
+def test_an_odd_number_of_blocks_over_two_groups(M, K, N, dtype):
+    """The second group of wavefronts has a block less: what it does instead adds nothing, also where the last block's
+    scales are infinite or its codes NaN."""
+    G = -(-K // 128)
+    xq = torch.full((M, K), 0x38, dtype=torch.uint8, device="cuda")  # ones
+    xs = torch.ones((M, G), device="cuda")
+    xs[1, G - 1] = float("inf")
+    xq[2, K - 1] = 0x7F
+    xs[M - 1, G - 1] = 0.0
+    wq = torch.full((N, K), 0x38, dtype=torch.uint8, device="cuda")
+    wq[1] = 0xB8  # minus ones
+    wq[2] = 0
+    wq[N - 1, K - 2] = 0xFF
+    ws = torch.ones((-(-N // 128), G), device="cuda")
+    ws[1, G - 1] = float("inf")  # channels 128 .. 255
+    got = layer(wq, ws).forward_a8(xq, xs, out_dtype=dtype).float()
+    assert got[0, 0] == K and got[0, 1] == -K and got[0, 2] == 0 and got[0, 300] == K  # (below 2^11 and whole 16s: exact in bf16)
+    assert got[1, 0] == float("inf") and got[1, 1] == -float("inf") and torch.isnan(got[1, 2])
+    assert torch.isnan(got[2]).all() and torch.isnan(got[:, N - 1]).all()
+    assert (got[3:M - 1, 128:256] == float("inf")).all() and (got[3:M - 1, 256:N - 1] == K).all()
+    rest = (G - 1) * 128
+    assert got[M - 1, 0] == rest and torch.isnan(got[M - 1, 128:256]).all() and (got[M - 1, 256:N - 1] == rest).all()
 
 
 def test_nothing_and_refusals():
