@@ -11,13 +11,13 @@
 // requested before the current one is reduced.  T grows with D (64 threads up to 1024 values, where no barrier is needed;
 // 256 up to 4096, 512 up to 8192, 1024 up to 16384) so that a thread holds at most 16 values of a row; longer rows are
 // walked in passes (the *_long kernels).
-// Measured, 8192 x 4096 in bf16: y in bf16 27 us (134 MB, 5.0 TB/s: what a copy moves), codes 24.3 - 25.3 (102 MB, 4.0 TB/s: the
+// Measured, 8192 x 4096 in bf16: y in bf16 24 us (134 MB, 5.6 TB/s, a copy's rate), codes 22.5 - 23.3 (102 MB, 4.4 TB/s: the
 // vector ALU, about 13 instructions a value, beside the two barriers a row); backward 38.3 + 4.8 (201 MB, 5.2 TB/s, and the
-// partials).  fp32 in and out: 49.8 us (5.4 TB/s).
+// partials).  fp32 in and out: 42 us (6.4 TB/s).
 //
 // 16 lanes hold 128 adjacent values: the block that shares a scale, so the quantised form needs one reduction over a DPP
 // row per vector and nothing else.  Rows whose length is no multiple of 8 are not 16-byte aligned: there a lane takes
-// every 16th value of its block instead of 8 adjacent ones, one load each.
+// every 16th value of its block instead of 8 adjacent ones, one load each (8192 x 4095 in bf16: 31.7 us).
 #include <algorithm>
 
 #include "nq_common.h"
