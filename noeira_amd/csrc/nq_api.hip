@@ -1384,6 +1384,7 @@ static int32_t check_norm(const char* what, const void* x, int32_t x_dtype, cons
     if (!x) return fail(NQ_ERR_INVALID, w + ": null x");
     if (((uintptr_t)x & 15) || ((uintptr_t)gamma & 15) || ((uintptr_t)beta & 15))
         return fail(NQ_ERR_INVALID, w + ": x, gamma and beta must be 16-byte aligned");
+    if (((uintptr_t)mean & 3) || ((uintptr_t)rstd & 3)) return fail(NQ_ERR_INVALID, w + ": mean and rstd must be 4-byte aligned");
     return NQ_OK;
 }
 
@@ -1429,6 +1430,8 @@ int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, co
         if (!x || !mean || !rstd || !gy || !gx) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: null pointer");
         if (((uintptr_t)x & 15) || ((uintptr_t)gy & 15) || ((uintptr_t)gx & 15))
             return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: x, gy and gx must be 16-byte aligned");
+        if (((uintptr_t)mean & 3) || ((uintptr_t)rstd & 3))
+            return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: mean and rstd must be 4-byte aligned");
         if ((gx == gy && gx_dtype != gy_dtype) || (gx == x && gx_dtype != x_dtype))
             return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: gx may be gy or x only where the types agree");
         const int64_t need = dgamma ? layer_norm_grad_partial_bytes(M, D) : 0;

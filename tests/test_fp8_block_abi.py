@@ -78,7 +78,7 @@ NORM = dict(x=64, xdt=L.DT_F32, gamma=64, beta=64, eps=1e-5, y=128, ydt=L.DT_F32
     (dict(D=0), "M >= 0 and D > 0"), (dict(M=-1), "M >= 0 and D > 0"), (dict(xdt=L.DT_I8), "x must be fp32 or bf16"),
     (dict(ydt=L.DT_I32), "y must be fp32 or bf16"), (dict(eps=-1.0), "eps must be"), (dict(eps=float("nan")), "eps must be"),
     (dict(eps=float("inf")), "eps must be"), (dict(mean=None), "together"), (dict(x=None), "null x"), (dict(x=68), "16-byte"),
-    (dict(gamma=68), "16-byte"), (dict(beta=68), "16-byte"), (dict(y=None), "16-byte"), (dict(y=132), "16-byte"),
+    (dict(mean=66), "4-byte"), (dict(rstd=65), "4-byte"), (dict(gamma=68), "16-byte"), (dict(beta=68), "16-byte"), (dict(y=None), "16-byte"), (dict(y=132), "16-byte"),
     (dict(y=64, ydt=L.DT_BF16), "where the types agree"),
 ])
 def test_layer_norm(change, words):
@@ -104,7 +104,7 @@ GRAD = dict(x=64, xdt=L.DT_F32, mean=64, rstd=64, gamma=64, gy=128, gydt=L.DT_F3
     (dict(D=0), L.NQ_ERR_INVALID, "M >= 0 and D > 0"), (dict(D=2 ** 26 + 1), L.NQ_ERR_INVALID, "2^26"), (dict(gydt=L.DT_I8), L.NQ_ERR_INVALID, "must be fp32 or bf16"),
     (dict(gxdt=7), L.NQ_ERR_INVALID, "must be fp32 or bf16"), (dict(dg=None), L.NQ_ERR_INVALID, "together"),
     (dict(dg=66), L.NQ_ERR_INVALID, "4-byte"), (dict(gy=None), L.NQ_ERR_INVALID, "null pointer"),
-    (dict(mean=None), L.NQ_ERR_INVALID, "null pointer"), (dict(gx=196), L.NQ_ERR_INVALID, "16-byte"),
+    (dict(mean=None), L.NQ_ERR_INVALID, "null pointer"), (dict(rstd=66), L.NQ_ERR_INVALID, "4-byte"), (dict(gx=196), L.NQ_ERR_INVALID, "16-byte"),
     (dict(gx=128, gxdt=L.DT_BF16), L.NQ_ERR_INVALID, "types agree"), (dict(gx=64, gxdt=L.DT_BF16), L.NQ_ERR_INVALID, "types agree"),
 ])
 def test_layer_norm_grad(change, code, words):
