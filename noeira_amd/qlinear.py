@@ -46,6 +46,10 @@ def _stream_ptr() -> int:
 _device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
+def _stream_now() -> int:
+    return _stream_ptr() if _raw_stream is None else _raw_stream(_device_now())
+
+
 def _need_gpu(target: str):
     if target != "gpu":
         raise L.NQError(L.NQ_ERR_UNSUPPORTED,
@@ -480,7 +484,7 @@ class FP8BlockLinear(_Layer):
             _check_dev(out, "FP8BlockLinear.forward_a8", "out", out_dtype, M * self.OUT)
         L.check(L.lib().nq_forward(self._h, x_codes.data_ptr(), L.DT_FP8_E4M3, x_scales.data_ptr(), out.data_ptr(),
                                    _TORCH_DT[out_dtype], M, _dev_ptr(bias), b_dt, L.EPI_RELU if epilogue == "relu" else L.EPI_NONE,
-                                   _stream_ptr()))
+                                   _stream_now()))
         return out
 
     def forward(self, x: torch.Tensor, bias=None, epilogue="none", out=None, out_dtype=torch.bfloat16):
@@ -501,8 +505,8 @@ class FP8BlockLinear(_Layer):
             grad_input = gy_codes.new_empty((M, self.IN), dtype=out_dtype)
         else:
             _check_dev(grad_input, "FP8BlockLinear.vjp_a8", "grad_input", out_dtype, M * self.IN)
-        L.check(L.lib().nq_grad_input_fp8_block(self._h, _dev_ptr(gy_codes), _dev_ptr(gy_scales), _dev_ptr(grad_input),
-                                                _TORCH_DT[out_dtype], M, _stream_ptr()))
+        L.check(L.lib().nq_grad_input_fp8_block(self._h, gy_codes.data_ptr(), gy_scales.data_ptr(), grad_input.data_ptr(),
+                                                _TORCH_DT[out_dtype], M, _stream_now()))
         return grad_input
 
     def vjp(self, forward_input: Optional[torch.Tensor], grad_output: torch.Tensor,
@@ -724,8 +728,8 @@ def quantize_rows_fp8_block(x: torch.Tensor, codes: Optional[torch.Tensor] = Non
         scales = x.new_empty((M, G), dtype=torch.float32)
     else:
         _check_dev(scales, "quantize_rows_fp8_block", "scales", torch.float32, M * G)
-    L.check(L.lib().nq_quantize_rows_fp8_block(_dev_ptr(x), _TORCH_DT[x.dtype], _dev_ptr(codes), _dev_ptr(scales), M, K,
-                                               _stream_ptr()))
+    L.check(L.lib().nq_quantize_rows_fp8_block(x.data_ptr(), _TORCH_DT[x.dtype], codes.data_ptr(), scales.data_ptr(), M, K,
+                                               _stream_now()))
     return codes, scales
 
 
