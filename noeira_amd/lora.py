@@ -103,12 +103,16 @@ def proj_fwd(base, x: torch.Tensor, adapter: "LoRAAdapter | None" = None, hessia
     its Hessian first (`HessianAccumulator.add`, hessian.mojo:41-77: `hessian` is a `noeira_amd.gptq.HessianAccumulator` or
     None); then the base linear; then the adapter's share, if the projection carries an unmerged one.  x: fp32 or
     bf16 [T, IN] on the device; returns fp32 [T, OUT].  `norm`: a `LayerNorm` ahead of all of that, or None; where only an
-    `FP8BlockLinear` reads its result, it hands over codes and block scales (`forward_fp8`) and nothing else is stored."""
+    `FP8BlockLinear` reads its result, it hands over codes and block scales (`forward_fp8`) and nothing else is stored.
+    An adapter or a Hessian beside such a layer reads the norm's fp32 result, the one that the codes are made from, so that
+    neither changes the layer's own share; every other layer takes the norm's result in x's type."""
     plain = adapter is None or adapter.merged
     if norm is not None:
         if isinstance(base, FP8BlockLinear) and plain and hessian is None:
             return base.forward_a8(*norm.forward_fp8(x), bias=bias, out=out, out_dtype=torch.float32)
-        x = norm.forward(x)
+        # (what a block-scaled layer quantises is the norm's fp32 result on either way: a rounding to bf16 ahead of it would move
+        # scales and codes when an adapter is attached, or a Hessian filled)
+        x = norm.forward(x, out_dtype=torch.float32 if isinstance(base, FP8BlockLinear) else None)
     if hessian is not None:
         hessian.add(x)
     if isinstance(base, FP8BlockLinear) and plain:

@@ -257,6 +257,26 @@ def test_projection_with_a_norm_and_an_adapter():
     assert torch.equal(proj_fwd(q, x, norm=norm), q.forward(xn))
 
 
+@pytest.mark.parametrize("M", [1, 21, 200])
+def test_projection_codes_do_not_depend_on_who_else_reads_the_norm(M):
+    """Over a block-scaled layer the rows' codes are the norm's fp32 result's, also for bf16 activations: an adapter of
+    zeros beside the layer, or a Hessian that is being filled, leaves the projection's bits as they are."""
+    from noeira_amd.gptq import HessianAccumulator
+    from noeira_amd.lora import LoRAAdapter, proj_fwd
+
+    norm, x, gen = inputs(M, 960, torch.bfloat16, 6)
+    lin = FP8BlockLinear(960, 320)
+    lin.set_weight(*R.random_weight(gen, 320, 960))
+    bias = torch.randn(320, generator=gen).cuda()
+    want = proj_fwd(lin, x, bias=bias, norm=norm)
+    assert torch.equal(want, lin.forward_a8(*norm.forward_fp8(x), bias=bias, out_dtype=torch.float32))
+    hessian = HessianAccumulator(960)
+    assert torch.equal(proj_fwd(lin, x, bias=bias, norm=norm, hessian=hessian), want)
+    assert hessian.rows == M
+    assert torch.equal(proj_fwd(lin, x, bias=bias, norm=norm, adapter=LoRAAdapter(960, 320, 8)), want)
+    assert torch.equal(proj_fwd(lin, x, bias=bias, norm=norm, adapter=LoRAAdapter(960, 320, 8), hessian=hessian), want)
+
+
 def test_two_graphs_at_once():
     """Two recorded backward steps of one norm keep their partial sums apart: replayed together on two streams, each
     returns the eager bits."""
