@@ -32,10 +32,10 @@ class LayerNorm:
         return cls(DIM, eps)
 
     def set_params(self, gamma, beta):
-        """fp32 [DIM] each: arrays or tensors; copied."""
+        """fp32 [DIM] each: arrays or tensors; copied (values only: no part of a graph that a tensor belongs to)."""
         new = []
         for name, v in (("gamma", gamma), ("beta", beta)):
-            t = v if isinstance(v, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(v, dtype=np.float32))
+            t = v.detach() if isinstance(v, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(v, dtype=np.float32))
             if tuple(t.shape) != (self.DIM,):
                 raise L.NQError(L.NQ_ERR_SIZE, f"LayerNorm.set_params: {name} is {list(t.shape)}, expected [{self.DIM}]")
             new.append(t)
