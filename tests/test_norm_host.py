@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from noeira_amd import NQError
+from noeira_amd import _lib as L
 from noeira_amd import norm as norm_module
 from noeira_amd import qlinear
 from noeira_amd.norm import LayerNorm
@@ -31,7 +31,7 @@ def test_parameters_are_copied_without_their_graph():
             assert not t.requires_grad and t.grad_fn is None
     norm.set_params(np.zeros(5), module.weight * 2)
     assert norm.beta.grad_fn is None and norm.beta[4] == 8 and not norm.gamma.any()
-    with pytest.raises(NQError, match="gamma is \\[4\\], expected \\[5\\]"):
+    with pytest.raises(L.NQError, match="gamma is \\[4\\], expected \\[5\\]"):
         norm.set_params(np.zeros(4), module.bias)
 
 
@@ -52,11 +52,11 @@ def test_counts_beyond_32_bits_are_refused(M, monkeypatch):
     for call in (lambda: norm.forward(x), lambda: norm.forward_train(x), lambda: norm.forward_fp8(x),
                  lambda: norm.vjp(x, stats, stats, x), lambda: qlinear.quantize_rows_fp8_block(x),
                  lambda: lin.forward_a8(codes, scales), lambda: lin.vjp_a8(codes, scales)):
-        with pytest.raises(NQError, match=f"{M} rows, at most 2\\^31 - 1"):
+        with pytest.raises(L.NQError, match=f"{M} rows, at most 2\\^31 - 1"):
             call()
-    with pytest.raises(NQError, match=f"{M} columns, at most"):
+    with pytest.raises(L.NQError, match=f"{M} columns, at most"):
         qlinear.quantize_rows_fp8_block(meta(1, M))
-    with pytest.raises(NQError, match="values in a row"):
+    with pytest.raises(L.NQError, match="values in a row"):
         LayerNorm(M)
-    with pytest.raises(NQError, match="DIM must be positive"):
+    with pytest.raises(L.NQError, match="DIM must be positive"):
         LayerNorm(0)
