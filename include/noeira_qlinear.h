@@ -174,6 +174,8 @@ int64_t nq_device_bytes(nq_handle h);
  * block's sum is off by at most 2.2e-4 of the sum of its terms' magnitudes, a
  * fraction of the output's own rounding); with an fp32 y on the bf16 ones, over
  * the exactly decoded codes, so that the sums are fp32 throughout.
+ * FP8_BLOCK takes every M and OUT that one of its kernels holds in a launch (the
+ * widest tiles reach beyond 10^9 rows into few channels); NQ_ERR_INVALID beyond.
  * x_scale is NULL otherwise.
  * y_dtype: F32 or BF16; I32 with x_dtype I8 returns the raw accumulators
  * (no scale, bias or epilogue).  bias may be NULL; bias_dtype F32 or BF16.

@@ -64,6 +64,13 @@ int32_t nq_diag_forward_gemm8(nq_handle h, const void* x, int32_t x_dtype, const
 int32_t nq_diag_forward_a16(nq_handle h, const void* x, int32_t x_dtype, void* y, int32_t y_dtype, int32_t M,
                             int32_t mw, int32_t nw, void* stream);
 
+/* What nq_forward takes for an FP8_BLOCK layer [OUT, IN] over M rows (nq_grad_input_fp8_block: with OUT and IN exchanged),
+ * decided on the host; nothing is launched and no device is needed (no counterpart in the reference).  form [5]: 0 the
+ * few-rows kernel, 1 the GEMM; rows and channels of a workgroup's tile; wavefronts (few rows) or groups of wavefronts
+ * (GEMM) that K is dealt over; the 256 x 256 tiles that a second launch does on 128 x 256 tiles.  Tests hold it that
+ * every form is run, and run deep.  NQ_ERR_INVALID where no form is one launch. */
+int32_t nq_diag_fp8_block_form(int32_t M, int32_t out_features, int32_t in_features, int32_t y_dtype, int32_t* form);
+
 #ifdef __cplusplus
 }
 #endif

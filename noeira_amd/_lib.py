@@ -40,6 +40,7 @@ EXPORTS = [
     "nq_set_weight_fp8_block", "nq_set_weight_fp8_block_dev", "nq_quantize_rows_fp8_block", "nq_grad_input_fp8_block",
     "nq_layer_norm", "nq_layer_norm_fp8_block", "nq_layer_norm_grad", "nq_layer_norm_grad_workspace_bytes",
     "nq_diag_mfma_rate", "nq_diag_stream_read", "nq_diag_gemm8_timeline", "nq_diag_forward_a16", "nq_diag_forward_gemm8",
+    "nq_diag_fp8_block_form",
 ]
 
 
@@ -194,6 +195,8 @@ def lib() -> C.CDLL:
     L.nq_layer_norm_grad_workspace_bytes.argtypes = [i32, i32]
     L.nq_layer_norm_grad.restype = i32
     L.nq_layer_norm_grad.argtypes = [p, i32, p, p, p, p, i32, p, i32, p, p, i32, i32, p, i64, p]
+    L.nq_diag_fp8_block_form.restype = i32
+    L.nq_diag_fp8_block_form.argtypes = [i32, i32, i32, i32, p]
     got = L.nq_abi_version()
     if got != ABI_VERSION:
         raise OSError(f"{LIB_NAME}: ABI version {got}, this package binds version {ABI_VERSION}")

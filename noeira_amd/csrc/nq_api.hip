@@ -1302,6 +1302,13 @@ int32_t nq_diag_forward_gemm8(nq_handle h, const void* x, int32_t x_dtype, const
     return launch_gemm8(a);
 }
 
+int32_t nq_diag_fp8_block_form(int32_t M, int32_t out_features, int32_t in_features, int32_t y_dtype, int32_t* form) {
+    if (M <= 0 || out_features <= 0 || in_features <= 0 || in_features % 16 != 0 || !form)
+        return fail(NQ_ERR_INVALID, "nq_diag_fp8_block_form: positive sizes, IN a multiple of 16, and room for the answer are needed");
+    if (y_dtype != NQ_DT_F32 && y_dtype != NQ_DT_BF16) return fail(NQ_ERR_INVALID, "nq_diag_fp8_block_form: y is fp32 or bf16");
+    return fp8_block_form(M, out_features, in_features, y_dtype, form);
+}
+
 int32_t nq_diag_forward_a16(nq_handle h, const void* x, int32_t x_dtype, void* y, int32_t y_dtype, int32_t M,
                             int32_t mw, int32_t nw, void* stream) {
     int32_t rc = check_handle(h, "nq_diag_forward_a16");

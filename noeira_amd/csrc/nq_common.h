@@ -228,6 +228,7 @@ int32_t launch_fp8_block_dequantize(const nq_layer* L, float* out, hipStream_t s
 int32_t launch_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* codes, float* scales, int32_t M, int32_t K,
                                        hipStream_t s);
 int32_t launch_fp8_block(const ForwardArgs& a);
+int32_t fp8_block_form(int32_t M, int32_t out, int32_t in, int32_t y_dtype, int32_t* form);  // nq_diag_fp8_block_form
 
 // nq_norm.hip: layer norm and its gradient
 struct NormArgs {

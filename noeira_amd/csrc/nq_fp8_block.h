@@ -75,9 +75,9 @@ struct BlockParams {
     SegTable seg;
 };
 
-// nq_fp8_block_gemm.hip
-bool fp8_block_gemm_applicable(const BlockParams& p);
-double fp8_block_gemm_estimate_us(const BlockParams& p);
+// nq_fp8_block_gemm.hip: whether the GEMM takes the call, and the time it is expected to take
+bool fp8_block_gemm_estimate_us(const BlockParams& p, double* us);
+void fp8_block_gemm_form(const BlockParams& p, int32_t* form);  // of a call that it takes: nq_diag_fp8_block_form
 int32_t launch_fp8_block_gemm(const BlockParams& p, hipStream_t s);
 
 }  // namespace nq

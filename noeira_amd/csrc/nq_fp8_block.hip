@@ -277,9 +277,8 @@ __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockPara
 
 template <int MT, int NT, int KW, int U>
 int32_t launch_tile(BlockParams p, hipStream_t s) {
-    p.tiles_m = (p.M + 16 * MT - 1) / (16 * MT);
-    const int64_t grid = (int64_t)p.tiles_m * ((p.N + 16 * NT - 1) / (16 * NT));
-    if (grid * 64 * KW > UINT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
+    p.tiles_m = (p.M - 1) / (16 * MT) + 1;
+    const int64_t grid = (int64_t)p.tiles_m * ((p.N - 1) / (16 * NT) + 1);  // (fits a launch: pick_shape)
     constexpr size_t lds = sizeof(float) * KW * 16 * MT * (16 * NT + 4);
     static LdsAttrOnce attr[2];
     if (p.y_dtype == NQ_DT_F32) {
@@ -303,20 +302,43 @@ struct Shape {
     int mt, nt;
 };
 constexpr Shape SHAPES[] = {{1, 1}, {1, 2}, {2, 2}, {2, 4}, {4, 4}};
+int64_t tile_workgroups(const BlockParams& p, const Shape& t) {
+    return (int64_t)((p.M - 1) / (16 * t.mt) + 1) * ((p.N - 1) / (16 * t.nt) + 1);
+}
+// K over 16 wavefronts where each keeps two blocks and more and few rows are read: such a call is bound by the loads
+// under way (1 row, 4096 -> 11008: 9.5 us against 9.9 on 8; 8 rows, 11008 -> 4096: 10.1 against 11.1; 16: 13.6 against 11.8)
+int tile_wavefronts(const BlockParams& p, const Shape& t) {
+    return t.mt * t.nt == 1 && (p.M == 1 ? p.G >= 32 : p.M <= 8 && p.G >= 64) ? 16 : 8;
+}
 double tile_estimate_us(const BlockParams& p, const Shape& t) {
-    const int64_t wgs = (int64_t)((p.M - 1) / (16 * t.mt) + 1) * ((p.N - 1) / (16 * t.nt) + 1);
+    const int64_t wgs = tile_workgroups(p, t);
     const double per_cu = (double)((wgs + 255) / 256), tiles = t.mt * t.nt;
     const double one = (double)p.K * (16.0 * (t.mt + t.nt) / 55e3 + (p.y_dtype == NQ_DT_F32 ? 9e-6 * tiles : 0.0));
     return 2.9 + 0.10 * tiles + per_cu * one + (per_cu - 1.0) * 0.19 * tiles;
 }
+// ... or null, where none is one launch of fewer than 2^32 threads
 const Shape* pick_shape(const BlockParams& p, double* us) {
     const Shape* best = nullptr;
     for (const Shape& t : SHAPES) {
         if (16 * (t.mt - 1) >= p.M) break;  // (no tile of rows that are not there)
+        if (tile_workgroups(p, t) * 64 * tile_wavefronts(p, t) > UINT32_MAX) continue;
         const double e = tile_estimate_us(p, t);
         if (!best || e < *us) best = &t, *us = e;
     }
     return best;
+}
+// the few-rows kernel's shape, or null for the GEMM
+int32_t pick_kernel(const BlockParams& p, const Shape** shape) {
+    double tile_us = 0.0;
+    *shape = pick_shape(p, &tile_us);
+    double gemm_us = 0.0;
+    if (!fp8_block_gemm_estimate_us(p, &gemm_us)) {
+        if (*shape) return NQ_OK;
+        return fail(NQ_ERR_INVALID, "FP8_BLOCK product: " + std::to_string(p.M) + " rows of " + std::to_string(p.N) +
+                                        " outputs are too many for one launch");
+    }
+    if (*shape && gemm_us < tile_us) *shape = nullptr;
+    return NQ_OK;
 }
 
 }  // namespace
@@ -364,6 +386,19 @@ int32_t launch_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* 
     return NQ_OK;
 }
 
+int32_t fp8_block_form(int32_t M, int32_t out, int32_t in, int32_t y_dtype, int32_t* form) {
+    BlockParams p{};
+    p.M = M, p.N = out, p.K = in, p.G = (in - 1) / FP8_BLOCK + 1, p.y_dtype = y_dtype;
+    const Shape* shape = nullptr;
+    if (const int32_t rc = pick_kernel(p, &shape)) return rc;
+    if (!shape) {
+        fp8_block_gemm_form(p, form);
+        return NQ_OK;
+    }
+    form[0] = 0, form[1] = 16 * shape->mt, form[2] = 16 * shape->nt, form[3] = tile_wavefronts(p, *shape), form[4] = 0;
+    return NQ_OK;
+}
+
 int32_t launch_fp8_block(const ForwardArgs& a) {
     const nq_layer* L = a.L;
     int device = -1;
@@ -379,14 +414,12 @@ int32_t launch_fp8_block(const ForwardArgs& a) {
     const uintptr_t line = a.y_dtype == NQ_DT_F32 ? 15 : 7;  // four channels of y
     p.vec = L->out % 4 == 0;
     for (int t = 0; t < a.seg.nseg; t++) p.vec = p.vec && ((uintptr_t)a.seg.y[t] & line) == 0;
-    double tile_us = 0.0;
-    const Shape* shape = pick_shape(p, &tile_us);
-    if (fp8_block_gemm_applicable(p) && fp8_block_gemm_estimate_us(p) < tile_us) return launch_fp8_block_gemm(p, a.stream);
+    const Shape* shape = nullptr;
+    if (const int32_t rc = pick_kernel(p, &shape)) return rc;
+    if (!shape) return launch_fp8_block_gemm(p, a.stream);
     switch (shape->mt * 8 + shape->nt) {
         case 1 * 8 + 1:
-            // K over 16 wavefronts where each keeps two blocks and more and few rows are read: such a call is bound by the loads
-            // under way (1 row, 4096 -> 11008: 9.5 us against 9.9 on 8; 8 rows, 11008 -> 4096: 10.1 against 11.1; 16: 13.6 against 11.8)
-            if (p.M == 1 ? p.G >= 32 : p.M <= 8 && p.G >= 64) return launch_tile<1, 1, 16, 2>(p, a.stream);
+            if (tile_wavefronts(p, *shape) == 16) return launch_tile<1, 1, 16, 2>(p, a.stream);
             return launch_tile<1, 1, 8, 2>(p, a.stream);
         case 1 * 8 + 2: return launch_tile<1, 2, 8, 2>(p, a.stream);
         case 2 * 8 + 2: return launch_tile<2, 2, 8, 2>(p, a.stream);

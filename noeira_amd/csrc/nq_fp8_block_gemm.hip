@@ -459,8 +459,7 @@ template <int BM, int BN, int WM, int WN, int NB, int KS, bool EXACT>
 int32_t launch(BlockParams p, hipStream_t s, int64_t grid = 0) {
     static LdsAttrOnce attr;
     p.tiles_m = (p.M - p.m_base - 1) / BM + 1, p.tiles_n = (p.N - p.n_base - 1) / BN + 1;
-    if (grid == 0) grid = (int64_t)p.tiles_m * p.tiles_n;
-    if (grid * 512 > INT32_MAX) return fail(NQ_ERR_INVALID, "nq_forward: M * OUT is too large for one launch");
+    if (grid == 0) grid = (int64_t)p.tiles_m * p.tiles_n;  // (fits a launch: pick)
     const void* kernel = reinterpret_cast<const void*>(&fp8_block_gemm_kernel<BM, BN, WM, WN, NB, KS, EXACT>);
     NQ_HIP(set_max_lds_once(attr, kernel, lds_bytes<BM, BN, NB, KS>()));
     hipLaunchKernelGGL((fp8_block_gemm_kernel<BM, BN, WM, WN, NB, KS, EXACT>), dim3((unsigned)grid), dim3(64 * WM * WN * KS), (lds_bytes<BM, BN, NB, KS>()), s, p);
@@ -511,34 +510,34 @@ double estimate256(int M, int N, int G, double off) {
     return rest ? estimate(F256, tiles - rest, G, off) + estimate(F128x256, 2 * rest, G, off) : estimate(F256, tiles, G, off);
 }
 
-// the form of lowest estimate and that estimate
+// the form of lowest estimate among those whose launch has fewer than 2^31 threads, and that estimate; null where none has,
+// or a tile's rows are beyond 32-bit offsets from its base
 const Form* pick(const BlockParams& p, double* us) {
+    if (p.M <= 64 || (int64_t)p.K * 256 >= ((int64_t)1 << 32)) return nullptr;
     const bool exact = p.y_dtype == NQ_DT_F32;
     const double off = p.N % (exact ? 4 : 8) == 0 ? 0.0 : exact ? 0.5 : 1.2;
-    const Form* best = exact ? &E256x128 : &F256;
-    *us = exact ? estimate(E256x128, p.M, p.N, p.G, off) : estimate256(p.M, p.N, p.G, off);
+    const Form* best = nullptr;
     const auto consider = [&](const Form& f) {
-        const double t = estimate(f, p.M, p.N, p.G, off);
-        if (t < *us) *us = t, best = &f;
+        if ((int64_t)((p.M - 1) / f.bm + 1) * ((p.N - 1) / f.bn + 1) * 512 > INT32_MAX) return;
+        const double t = &f == &F256 ? estimate256(p.M, p.N, p.G, off) : estimate(f, p.M, p.N, p.G, off);
+        if (!best || t < *us) *us = t, best = &f;
     };
     if (exact)
-        consider(E128), consider(E64), consider(E64K2);
+        consider(E256x128), consider(E128), consider(E64), consider(E64K2);
     else
-        consider(F128x256), consider(F128), consider(F64K2);
+        consider(F256), consider(F128x256), consider(F128), consider(F64K2);
     return best;
 }
 
 }  // namespace
 
-bool fp8_block_gemm_applicable(const BlockParams& p) {
-    // 32-bit offsets from a tile's base
-    return p.M > 64 && (int64_t)p.K * 256 < ((int64_t)1 << 32);
-}
+bool fp8_block_gemm_estimate_us(const BlockParams& p, double* us) { return pick(p, us) != nullptr; }
 
-double fp8_block_gemm_estimate_us(const BlockParams& p) {
+void fp8_block_gemm_form(const BlockParams& p, int32_t* form) {
     double us;
-    pick(p, &us);
-    return us;
+    const Form* f = pick(p, &us);
+    form[0] = 1, form[1] = f->bm, form[2] = f->bn, form[3] = f == &E64K2 || f == &F64K2 ? 2 : 1;
+    form[4] = f == &F256 ? (int32_t)leftover(p.M, p.N) : 0;
 }
 
 int32_t launch_fp8_block_gemm(const BlockParams& p, hipStream_t s) {
