@@ -43,6 +43,71 @@ def test_what_fits_no_launch_is_refused(M, N, dtype):
             form(M, K, N, dtype)
 
 
+# every kernel and tile there is, as form() names them; the last: with tiles left to the second launch
+FEW = [(0, 16, 16, 8), (0, 16, 16, 16), (0, 16, 32, 8), (0, 32, 32, 8), (0, 32, 64, 8), (0, 64, 64, 8)]
+FORMS = {"f32": FEW + [(1, 64, 128, 1), (1, 64, 128, 2), (1, 128, 128, 1), (1, 256, 128, 1)],
+         "bf16": FEW + [(1, 64, 128, 2), (1, 128, 128, 1), (1, 128, 256, 1), (1, 256, 256, 1), (1, 256, 256, 1, "and rest")]}
+# 65 blocks of K, 16 values in the last, into an odd number of channels; 32 whole blocks into whole tiles.  The GEMM's stage
+# buffers (two to four) and its three buffers of four stages' scales are taken in turn: from 13 stages of a group on
+# (26 blocks, where two groups share them) a buffer of scales is filled a second time.  A few-rows wavefront of eight
+# walks beyond its first four blocks from 33 on.
+DEEP = [(17, 8208, 1001), (3, 8208, 1001), (17, 8208, 4001), (300, 8208, 513), (40, 8208, 8101), (500, 8208, 1301), (777, 8208, 2567),
+        (321, 8208, 3001), (2045, 8208, 2567), (1300, 8208, 8101), (2304, 8208, 8101), (1030, 8208, 3333),
+        (400, 4096, 2560), (512, 4096, 2048), (1024, 4096, 4096), (2048, 4096, 2560), (2304, 4096, 4096), (4096, 4096, 4352)]
+
+
+def kinds(K, dtype):
+    got = set()
+    for M, k, N in DEEP:
+        if k == K:
+            f = form(M, K, N, dtype)
+            got.add(f[:4] + ("and rest",) if f[4] else f[:4])
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_deep_cases_run_every_form(dtype):
+    """A retuned choice must not leave a form without a deep case."""
+    assert kinds(8208, dtype) == set(FORMS[dtype])
+    assert kinds(4096, dtype) >= {f for f in FORMS[dtype] if f[0] == 1}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", DEEP)
+def test_deep_products(M, K, N, dtype):
+    gen = torch.Generator().manual_seed(M + K + N)
+    xq, xs = R.random_rows(gen, M, K)
+    wq, ws = R.random_weight(gen, N, K)
+    lin = FP8BlockLinear(K, N)
+    lin.set_weight(wq, ws)
+    bias = torch.randn(N, generator=gen).cuda()
+    store = torch.full((M * N + 64,), 77.0, dtype=DTYPES[dtype], device="cuda")
+    got = lin.forward_a8(xq, xs, bias=bias, out=store[: M * N].view(M, N), out_dtype=DTYPES[dtype])
+    x, w = R.rows(xq, xs), R.matrix(wq, ws)
+    y = x @ w.t() + bias.double()
+    R.assert_within(got, y, R.product_bound(x, w, y, bias.double(), DTYPES[dtype]), "y")
+    assert (store[M * N:] == 77.0).all()
+    for _ in range(3):
+        assert torch.equal(lin.forward_a8(xq, xs, bias=bias, out_dtype=DTYPES[dtype]), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(3, 1008, 8208), (300, 528, 8208), (321, 3008, 8208), (2045, 2576, 8208)])
+def test_deep_gradients(M, K, N, dtype):
+    """gx[M, K] from gy[M, N]: blocks of N, the kernels of the product."""
+    gen = torch.Generator().manual_seed(M + K)
+    wq, ws = R.random_weight(gen, N, K)
+    lin = FP8BlockLinear(K, N, grad=True)
+    lin.set_weight(wq, ws)
+    gq, gs = R.random_rows(gen, M, N)
+    g, w = R.rows(gq, gs), R.matrix(wq, ws)
+    want = g @ w
+    got = lin.vjp_a8(gq, gs, out_dtype=DTYPES[dtype])
+    R.assert_within(got, want, R.product_bound(g, w.t(), want, None, DTYPES[dtype]), "gx")
+
+
 def test_arguments():
     got = (C.c_int32 * 5)()
     for args in ((0, 16, 16, 0, got), (1, 0, 16, 0, got), (1, 16, 24, 0, got), (1, 16, 16, 0, None), (1, 16, 16, L.DT_I8, got)):
