@@ -174,10 +174,13 @@ int64_t nq_device_bytes(nq_handle h);
  * add eight adjacent products under the largest one's exponents and drop what
  * lies below 2^-13 of those: a block's sum is off by 1.3e-5 of the sums' root
  * mean square for codes of N(0, 1) values, and at worst by 7 * 2^-13 = 8.5e-4
- * of the sum of its terms' magnitudes (up to 64 times that of a group whose
- * codes are subnormal where the others are large).  So a y whose terms cancel
- * can be off by more than its own rounding.  With an fp32 y the bf16 matrix
+ * of the sum of its terms' magnitudes (up to 64 times that share of a group whose
+ * largest product is one of subnormal codes).  So a y whose terms cancel can be
+ * off by more than its own rounding.  With an fp32 y the bf16 matrix
  * cores multiply the exactly decoded codes and the sums are fp32 throughout.
+ * A block's two scales are multiplied first, in fp32: below 2^-126 their product
+ * loses precision, from 2^128 on it is infinite (and a sum of zero times that a
+ * NaN).
  * FP8_BLOCK takes every M and OUT that one of its kernels holds in a launch (the
  * widest tiles reach beyond 10^9 rows into few channels); NQ_ERR_INVALID beyond.
  * x_scale is NULL otherwise.

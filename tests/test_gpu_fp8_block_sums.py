@@ -70,3 +70,17 @@ def test_codes_of_every_magnitude(M, K):
     wq[:, half:] = wq[:, :half] ^ 0x80
     wq[torch.rand(130, K, generator=gen) < 0.05] = 0x01
     check(xq, xs, wq, ws)
+
+
+@pytest.mark.parametrize("M", [40, 300])
+@pytest.mark.parametrize("ex,ew", [(100, -110), (-100, 90), (-126, 20), (-60, -60), (50, 40), (-110, -10)])
+def test_scales_of_every_magnitude(M, ex, ew):
+    """A block's two scales are multiplied first, in fp32: wherever that product is a normal number, however far the two are
+    apart, the result keeps its relative precision."""
+    gen = torch.Generator().manual_seed(M + ex)
+    K, N = 272, 130
+    xq, xs = R.random_rows(gen, M, K)
+    wq, ws = R.random_weight(gen, N, K)
+    xs = ((1 + torch.rand(xs.shape, generator=gen)).double() * 2.0 ** ex).float().cuda()
+    ws = ((1 + torch.rand(ws.shape, generator=gen)).double() * 2.0 ** ew).float().cuda()
+    check(xq, xs, wq, ws)
