@@ -29,6 +29,15 @@ hipError_t set_max_lds_once(LdsAttrOnce& st, const void* kernel, size_t bytes) {
     return e;
 }
 
+// behind an entry point: what it could not allocate for (a sentence, mostly) ends as a status.  (The sentence here is short
+// enough for a string's own storage.)
+static int32_t out_of_memory() {
+    g_last_error = "out of memory";
+    return NQ_ERR_INVALID;
+}
+#define NQ_NO_THROW \
+    catch (...) { return out_of_memory(); }
+
 int32_t fail_hip(hipError_t e, const char* what) {
     g_last_error = std::string("HIP error ") + hipGetErrorName(e) + " (" + hipGetErrorString(e) + ") in " + what;
     return NQ_ERR_HIP;
@@ -138,7 +147,7 @@ int64_t nq_last_error(char* buf, int64_t n) {
 }
 
 int32_t nq_create(nq_handle* out, int32_t format, int32_t in_features, int32_t out_features, int32_t group,
-                  int32_t flags) {
+                  int32_t flags) try {
     if (!out) return fail(NQ_ERR_INVALID, "nq_create: null output handle");
     *out = nullptr;
     if (format < NQ_FMT_Q4_0 || format > NQ_FMT_FP8_BLOCK)
@@ -178,7 +187,7 @@ int32_t nq_create(nq_handle* out, int32_t format, int32_t in_features, int32_t o
     L->keep_grad = (flags & NQ_FLAG_GRAD) != 0;
     *out = L;
     return NQ_OK;
-}
+} NQ_NO_THROW
 
 int32_t nq_destroy(nq_handle h) {
     if (!h) return NQ_OK;
@@ -424,13 +433,13 @@ static int32_t set_weight_fp8_block(nq_handle h, const uint8_t* codes, const flo
     return NQ_OK;
 }
 
-int32_t nq_set_weight_fp8_block(nq_handle h, const uint8_t* codes_host, const float* scales_host, void* stream) {
+int32_t nq_set_weight_fp8_block(nq_handle h, const uint8_t* codes_host, const float* scales_host, void* stream) try {
     return set_weight_fp8_block(h, codes_host, scales_host, true, stream);
-}
+} NQ_NO_THROW
 
-int32_t nq_set_weight_fp8_block_dev(nq_handle h, const uint8_t* codes, const float* scales, void* stream) {
+int32_t nq_set_weight_fp8_block_dev(nq_handle h, const uint8_t* codes, const float* scales, void* stream) try {
     return set_weight_fp8_block(h, codes, scales, false, stream);
-}
+} NQ_NO_THROW
 
 int64_t nq_blocks_bytes(nq_handle h) {
     if (!h) return 0;
@@ -655,7 +664,7 @@ int32_t forward_impl(nq_handle h, const void* x, int32_t x_dtype, const float* x
 }  // namespace
 
 int32_t nq_forward(nq_handle h, const void* x, int32_t x_dtype, const float* x_scale, void* y, int32_t y_dtype,
-                   int32_t M, const void* bias, int32_t bias_dtype, int32_t epilogue, void* stream) {
+                   int32_t M, const void* bias, int32_t bias_dtype, int32_t epilogue, void* stream) try {
     int32_t rc = check_handle(h, "nq_forward");
     if (rc) return rc;
     if ((rc = need_loaded(h, "forward"))) return rc;
@@ -665,9 +674,9 @@ int32_t nq_forward(nq_handle h, const void* x, int32_t x_dtype, const float* x_s
     SegTable seg{};
     seg.nseg = 1, seg.end[0] = h->out, seg.y[0] = y;
     return forward_impl(h, x, x_dtype, x_scale, seg, y_dtype, M, bias, bias_dtype, epilogue, stream);
-}
+} NQ_NO_THROW
 
-int32_t nq_fuse_rows(nq_handle* out, const nq_handle* layers, int32_t n, void* stream) {
+int32_t nq_fuse_rows(nq_handle* out, const nq_handle* layers, int32_t n, void* stream) try {
     if (!out) return fail(NQ_ERR_INVALID, "nq_fuse_rows: null output handle");
     *out = nullptr;
     if (!layers || n < 1 || n > 4) return fail(NQ_ERR_INVALID, "nq_fuse_rows: between 1 and 4 layers can be fused");
@@ -691,6 +700,12 @@ int32_t nq_fuse_rows(nq_handle* out, const nq_handle* layers, int32_t n, void* s
     const nq_layer* a = layers[0];
     nq_layer* F = new (std::nothrow) nq_layer();
     if (!F) return fail(NQ_ERR_INVALID, "nq_fuse_rows: out of host memory");
+    try {
+        F->seg_end.reserve((size_t)n);
+    } catch (const std::bad_alloc&) {
+        delete F;
+        return fail(NQ_ERR_INVALID, "nq_fuse_rows: out of host memory");
+    }
     F->format = a->format, F->in = a->in, F->out = (int32_t)rows, F->group = a->group, F->groups = a->groups;
     F->scale = a->scale, F->row_bytes = a->row_bytes, F->device = a->device;
     F->no_tile_copy = a->no_tile_copy, F->prefer_tile = a->prefer_tile;
@@ -782,7 +797,7 @@ int32_t nq_fuse_rows(nq_handle* out, const nq_handle* layers, int32_t n, void* s
     F->loaded = true;
     *out = F;
     return NQ_OK;
-}
+} NQ_NO_THROW
 
 int32_t nq_fuse_glu(nq_handle* out, nq_handle gate, nq_handle up, void* stream) {
     if (!out) return fail(NQ_ERR_INVALID, "nq_fuse_glu: null output handle");
@@ -856,7 +871,7 @@ int32_t nq_fused_parts(nq_handle h) {
 
 int32_t nq_forward_fused(nq_handle h, const void* x, int32_t x_dtype, const float* x_scale, void* const* ys,
                          int32_t n_ys, int32_t y_dtype, int32_t M, const void* bias, int32_t bias_dtype,
-                         int32_t epilogue, void* stream) {
+                         int32_t epilogue, void* stream) try {
     int32_t rc = check_handle(h, "nq_forward_fused");
     if (rc) return rc;
     if ((rc = need_loaded(h, "forward"))) return rc;
@@ -875,7 +890,7 @@ int32_t nq_forward_fused(nq_handle h, const void* x, int32_t x_dtype, const floa
         if (!ys[t]) return fail(NQ_ERR_INVALID, "nq_forward: null x or y");
     }
     return forward_impl(h, x, x_dtype, x_scale, seg, y_dtype, M, bias, bias_dtype, epilogue, stream);
-}
+} NQ_NO_THROW
 
 int32_t nq_dequantize(nq_handle h, float* out_dev, int64_t n_values, void* stream) {
     int32_t rc = check_handle(h, "nq_dequantize");
@@ -1302,12 +1317,12 @@ int32_t nq_diag_forward_gemm8(nq_handle h, const void* x, int32_t x_dtype, const
     return launch_gemm8(a);
 }
 
-int32_t nq_diag_fp8_block_form(int32_t M, int32_t out_features, int32_t in_features, int32_t y_dtype, int32_t* form) {
+int32_t nq_diag_fp8_block_form(int32_t M, int32_t out_features, int32_t in_features, int32_t y_dtype, int32_t* form) try {
     if (M <= 0 || out_features <= 0 || in_features <= 0 || in_features % 16 != 0 || !form)
         return fail(NQ_ERR_INVALID, "nq_diag_fp8_block_form: positive sizes, IN a multiple of 16, and room for the answer are needed");
     if (y_dtype != NQ_DT_F32 && y_dtype != NQ_DT_BF16) return fail(NQ_ERR_INVALID, "nq_diag_fp8_block_form: y is fp32 or bf16");
     return fp8_block_form(M, out_features, in_features, y_dtype, form);
-}
+} NQ_NO_THROW
 
 int32_t nq_diag_forward_a16(nq_handle h, const void* x, int32_t x_dtype, void* y, int32_t y_dtype, int32_t M,
                             int32_t mw, int32_t nw, void* stream) {
@@ -1343,7 +1358,7 @@ int32_t nq_quantize_rows_i8(const void* x, int32_t x_dtype, int8_t* q, float* sc
 }
 
 int32_t nq_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* codes, float* scales, int32_t M, int32_t K,
-                                   void* stream) {
+                                   void* stream) try {
     if (M < 0 || K <= 0) return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: M >= 0 and K > 0 are required");
     if (x_dtype != NQ_DT_F32 && x_dtype != NQ_DT_BF16)
         return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: x must be fp32 or bf16");
@@ -1352,10 +1367,10 @@ int32_t nq_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* code
     if (((uintptr_t)x & 15) || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3))
         return fail(NQ_ERR_INVALID, "nq_quantize_rows_fp8_block: x and codes must be 16-byte and scales 4-byte aligned");
     return launch_quantize_rows_fp8_block(x, x_dtype, codes, scales, M, K, (hipStream_t)stream);
-}
+} NQ_NO_THROW
 
 int32_t nq_grad_input_fp8_block(nq_handle h, const uint8_t* gy, const float* gy_scale, void* gx, int32_t gx_dtype, int32_t M,
-                                void* stream) {
+                                void* stream) try {
     int32_t rc = check_handle(h, "nq_grad_input_fp8_block");
     if (rc) return rc;
     if ((rc = need_loaded(h, "vjp"))) return rc;
@@ -1377,26 +1392,25 @@ int32_t nq_grad_input_fp8_block(nq_handle h, const uint8_t* gy, const float* gy_
     seg.nseg = 1, seg.end[0] = T.out, seg.y[0] = gx;
     const ForwardArgs a{&T, gy, NQ_DT_FP8_E4M3, gy_scale, gx, gx_dtype, M, nullptr, NQ_DT_F32, NQ_EPI_NONE, (hipStream_t)stream, seg};
     return launch_fp8_block(a);
-}
+} NQ_NO_THROW
 
 // what the two forms of the norm's forward ask of their common arguments
 static int32_t check_norm(const char* what, const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps,
                           const float* mean, const float* rstd, int32_t M, int32_t D) {
-    const std::string w(what);
-    if (M < 0 || D <= 0) return fail(NQ_ERR_INVALID, w + ": M >= 0 and D > 0 are required");
-    if (x_dtype != NQ_DT_F32 && x_dtype != NQ_DT_BF16) return fail(NQ_ERR_INVALID, w + ": x must be fp32 or bf16");
-    if (!(eps >= 0.0f) || eps > 3.402823466e38f) return fail(NQ_ERR_INVALID, w + ": eps must be finite and not negative");
-    if ((mean == nullptr) != (rstd == nullptr)) return fail(NQ_ERR_INVALID, w + ": mean and rstd are given together or not at all");
+    if (M < 0 || D <= 0) return fail(NQ_ERR_INVALID, std::string(what) + ": M >= 0 and D > 0 are required");
+    if (x_dtype != NQ_DT_F32 && x_dtype != NQ_DT_BF16) return fail(NQ_ERR_INVALID, std::string(what) + ": x must be fp32 or bf16");
+    if (!(eps >= 0.0f) || eps > 3.402823466e38f) return fail(NQ_ERR_INVALID, std::string(what) + ": eps must be finite and not negative");
+    if ((mean == nullptr) != (rstd == nullptr)) return fail(NQ_ERR_INVALID, std::string(what) + ": mean and rstd are given together or not at all");
     if (M == 0) return NQ_OK;
-    if (!x) return fail(NQ_ERR_INVALID, w + ": null x");
+    if (!x) return fail(NQ_ERR_INVALID, std::string(what) + ": null x");
     if (((uintptr_t)x & 15) || ((uintptr_t)gamma & 15) || ((uintptr_t)beta & 15))
-        return fail(NQ_ERR_INVALID, w + ": x, gamma and beta must be 16-byte aligned");
-    if (((uintptr_t)mean & 3) || ((uintptr_t)rstd & 3)) return fail(NQ_ERR_INVALID, w + ": mean and rstd must be 4-byte aligned");
+        return fail(NQ_ERR_INVALID, std::string(what) + ": x, gamma and beta must be 16-byte aligned");
+    if (((uintptr_t)mean & 3) || ((uintptr_t)rstd & 3)) return fail(NQ_ERR_INVALID, std::string(what) + ": mean and rstd must be 4-byte aligned");
     return NQ_OK;
 }
 
 int32_t nq_layer_norm(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps, void* y,
-                      int32_t y_dtype, float* mean, float* rstd, int32_t M, int32_t D, void* stream) {
+                      int32_t y_dtype, float* mean, float* rstd, int32_t M, int32_t D, void* stream) try {
     const int32_t rc = check_norm("nq_layer_norm", x, x_dtype, gamma, beta, eps, mean, rstd, M, D);
     if (rc) return rc;
     if (y_dtype != NQ_DT_F32 && y_dtype != NQ_DT_BF16) return fail(NQ_ERR_INVALID, "nq_layer_norm: y must be fp32 or bf16");
@@ -1405,10 +1419,10 @@ int32_t nq_layer_norm(const void* x, int32_t x_dtype, const float* gamma, const 
     if (y == x && y_dtype != x_dtype) return fail(NQ_ERR_INVALID, "nq_layer_norm: y may be x only where the types agree");
     NormArgs a{x, x_dtype, gamma, beta, eps, y, y_dtype, nullptr, nullptr, mean, rstd, M, D};
     return launch_layer_norm(a, (hipStream_t)stream);
-}
+} NQ_NO_THROW
 
 int32_t nq_layer_norm_fp8_block(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps,
-                                uint8_t* codes, float* scales, float* mean, float* rstd, int32_t M, int32_t D, void* stream) {
+                                uint8_t* codes, float* scales, float* mean, float* rstd, int32_t M, int32_t D, void* stream) try {
     const int32_t rc = check_norm("nq_layer_norm_fp8_block", x, x_dtype, gamma, beta, eps, mean, rstd, M, D);
     if (rc) return rc;
     if (M == 0) return NQ_OK;
@@ -1416,7 +1430,7 @@ int32_t nq_layer_norm_fp8_block(const void* x, int32_t x_dtype, const float* gam
         return fail(NQ_ERR_INVALID, "nq_layer_norm_fp8_block: codes (16-byte aligned) and scales (4-byte) are needed");
     NormArgs a{x, x_dtype, gamma, beta, eps, nullptr, NQ_DT_F32, codes, scales, mean, rstd, M, D};
     return launch_layer_norm(a, (hipStream_t)stream);
-}
+} NQ_NO_THROW
 
 int64_t nq_layer_norm_grad_workspace_bytes(int32_t M, int32_t D) {
     return M <= 0 || D <= 0 ? 0 : layer_norm_grad_partial_bytes(M, D);
@@ -1424,7 +1438,7 @@ int64_t nq_layer_norm_grad_workspace_bytes(int32_t M, int32_t D) {
 
 int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, const float* rstd, const float* gamma,
                            const void* gy, int32_t gy_dtype, void* gx, int32_t gx_dtype, float* dgamma, float* dbeta,
-                           int32_t M, int32_t D, void* workspace, int64_t workspace_bytes, void* stream) {
+                           int32_t M, int32_t D, void* workspace, int64_t workspace_bytes, void* stream) try {
     if (M < 0 || D <= 0) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: M >= 0 and D > 0 are required");
     if (D > 1 << 26) return fail(NQ_ERR_INVALID, "nq_layer_norm_grad: rows of more than 2^26 values");
     for (int32_t t : {x_dtype, gy_dtype, gx_dtype})
@@ -1447,7 +1461,7 @@ int32_t nq_layer_norm_grad(const void* x, int32_t x_dtype, const float* mean, co
     }
     const NormGradArgs a{x, gy, gx, x_dtype, gy_dtype, gx_dtype, mean, rstd, gamma, dgamma, dbeta, M, D, reinterpret_cast<float*>(workspace)};
     return launch_layer_norm_grad(a, (hipStream_t)stream);
-}
+} NQ_NO_THROW
 
 int32_t nq_cast_pad_bf16(const float* src, uint16_t* dst, int32_t rows, int32_t cols, int32_t cols_pad,
                          void* stream) {
