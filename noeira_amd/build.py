@@ -46,6 +46,11 @@ NO_SPILL = {"nq_gemv_tile.hip": ("gemv_tile4i_kernel", "gemv_tile4_rows_kernel",
 # No loads under way in registers here, but a register budget that is full to the last few, in a loop where spills have
 # cost ten times the call.
 NO_SPILL_TUNED = {"nq_fp8_block_gemm.hip": ("fp8_block_gemm_kernel",)}
+# The norm's kernels hold a row in registers and use no scratch memory, but for the rows of 8193 to 16384 values: 16 per
+# thread of x, gy, gamma and both sums are a few registers more than 16 wavefronts per CU leave (bytes per lane as
+# compiled, by the first entry that a kernel's name holds; the build refuses more).
+SCRATCH_LIMITS = {"nq_norm.hip": (("layer_norm_grad_kernelILi1024ELi2E", 84), ("layer_norm_kernelILi1024ELi2ELb0ELb0E", 28),
+                                  ("layer_norm_", 0))}
 # The large-tile GEMM is held to nearly the same rule for its speed: 256 accumulators per lane leave its epilogue a
 # tight budget, and a variant that spilled there has cost 60 % of the call before.  One or two values parked in scratch
 # memory ahead of the K loop and fetched back in the epilogue are tolerated (SPEED_SCRATCH_BYTES per lane); the K loop
@@ -68,6 +73,22 @@ def _spilling_kernels(remarks: str, names, allow_bytes: int = 0) -> list:
             limit = allow_bytes if m.group(1).startswith("ScratchSize") else allow_bytes // 4
             if int(m.group(2)) > limit:
                 out.append(cur)
+    return out
+
+
+def _beyond_scratch(remarks: str, limits) -> list:
+    """From the compiler's kernel-resource-usage remarks: (kernel, bytes per lane) where the first of `limits` (part of a
+    kernel's name, bytes) that fits allows fewer."""
+    out, cur, allowed = [], None, 0
+    for l in remarks.splitlines():
+        m = re.search(r"remark: Function Name: (\S+)", l)
+        if m:
+            cur = m.group(1)
+            allowed = next((b for part, b in limits if part in cur), None)
+            continue
+        m = re.search(r"remark:\s+ScratchSize \[bytes/lane\]: (\d+)", l)
+        if m and cur and allowed is not None and int(m.group(1)) > allowed:
+            out.append((cur, int(m.group(1))))
     return out
 
 
@@ -230,18 +251,22 @@ def _compile(src: str, force: bool) -> str:
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= newest:
         return obj
     guarded = NO_SPILL.get(src) or NO_SPILL_FOR_SPEED.get(src) or NO_SPILL_TUNED.get(src)
-    cmd = [HIPCC] + FLAGS + EXTRA_FLAGS.get(src, []) + (["-Rpass-analysis=kernel-resource-usage"] if guarded else []) + ["-c", path, "-o", obj]
+    cmd = [HIPCC] + FLAGS + EXTRA_FLAGS.get(src, []) + (["-Rpass-analysis=kernel-resource-usage"] if guarded or src in SCRATCH_LIMITS else []) + ["-c", path, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src}:\n{r.stdout}\n{r.stderr}")
     err = r.stderr
-    if guarded:
-        spilled = _spilling_kernels(err, guarded, SPEED_SCRATCH_BYTES if src in NO_SPILL_FOR_SPEED else 0)
+    if guarded or src in SCRATCH_LIMITS:
+        spilled = _spilling_kernels(err, guarded, SPEED_SCRATCH_BYTES if src in NO_SPILL_FOR_SPEED else 0) if guarded else []
+        beyond = _beyond_scratch(err, SCRATCH_LIMITS.get(src, ()))
         err = "\n".join(l for l in err.splitlines() if "kernel-resource-usage" not in l and not re.match(r"^\s+(\d+ \||\|)", l))
         if spilled:
             os.remove(obj)
             raise RuntimeError(f"{src}: kernels that keep loads under way in registers, or whose register budget is tuned, "
                                f"must not spill: {spilled}")
+        if beyond:
+            os.remove(obj)
+            raise RuntimeError(f"{src}: kernels that use more scratch memory per lane than they are known to: {beyond}")
     if src in NO_SPILL_FOR_SPEED:
         cmd = [HIPCC] + FLAGS + EXTRA_FLAGS.get(src, []) + ["--cuda-device-only", "-S", path, "-o", obj + ".s"]
         r = subprocess.run(cmd, capture_output=True, text=True)

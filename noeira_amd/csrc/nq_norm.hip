@@ -270,7 +270,9 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(const NormArgs a)
 // partials (one workgroup per CU) are left to add: 2 D fp32 each, 8 MB for D = 4096 against 200 of rows at M = 8192.
 // A thread holds 8 values of x, gy, gamma and both sums and the next row's raw 8 (90 registers of the 128 that 16
 // wavefronts per CU leave it); with 16 of each it spilled (8192 x 4096 in bf16: 76 us a call against 40).  Rows of more than
-// 8192 values have 16 per thread and do without the early request (AHEAD).
+// 8192 values have 16 per thread and do without the early request (AHEAD), and still put a few of them in scratch memory:
+// 12 - 20 bytes per lane, 84 where the length is no multiple of 8 (noeira_amd/build.py holds them to that).  8192 x 11008
+// takes 133 us in bf16 (4.1 TB/s) and 219 in fp32 (4.9), 2048 x 16384 66 and 105.
 template <int T, int NV, bool XB, bool GB, bool VEC>
 __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(const NormGradArgs a, int32_t rounds) {
     extern __shared__ __attribute__((aligned(16))) float meet[];  // [2][T * 8 * NV] where there are teams to meet
