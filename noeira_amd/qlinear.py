@@ -472,9 +472,12 @@ class FP8BlockLinear(_Layer):
         _check_dev(scales, what, "the scales", torch.float32, M * (-(-K // 128)))
         return M
 
-    def forward_a8(self, x_codes, x_scales, bias=None, epilogue="none", out=None, out_dtype=torch.bfloat16):
-        """x_codes: e4m3fn (or uint8) [M, IN]; x_scales: fp32 [M, ceil(IN/128)]."""
+    def forward_a8(self, x_codes, x_scales, bias=None, epilogue="none", out=None, out_dtype=None):
+        """x_codes: e4m3fn (or uint8) [M, IN]; x_scales: fp32 [M, ceil(IN/128)].  y is of `out_dtype` (fp32 or bf16), or
+        without one of `out`'s type, bf16 where neither is given."""
         M = self._codes(x_codes, x_scales, self.IN, "FP8BlockLinear.forward_a8")
+        if out_dtype is None:
+            out_dtype = torch.bfloat16 if out is None else out.dtype
         if out_dtype not in _TORCH_DT:
             raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.forward_a8: y must be fp32 or bf16")
         if epilogue not in ("none", "relu"):
@@ -494,18 +497,22 @@ class FP8BlockLinear(_Layer):
                                    _stream_now()))
         return out
 
-    def forward(self, x: torch.Tensor, bias=None, epilogue="none", out=None, out_dtype=torch.bfloat16):
-        """fp32 or bf16 activations: quantised per row and block of 128, then the product (two launches)."""
+    def forward(self, x: torch.Tensor, bias=None, epilogue="none", out=None, out_dtype=None):
+        """fp32 or bf16 activations: quantised per row and block of 128, then the product (two launches); `out` and
+        `out_dtype` as in `forward_a8`."""
         if x.dtype not in _TORCH_DT:
             raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.forward: x must be fp32 or bf16")
         M = _check_x(x, self.IN, "FP8BlockLinear.forward")
         return self.forward_a8(*quantize_rows_fp8_block(x.view(M, self.IN)), bias=bias, epilogue=epilogue, out=out,
                                out_dtype=out_dtype)
 
-    def vjp_a8(self, gy_codes, gy_scales, grad_input: Optional[torch.Tensor] = None, out_dtype=torch.float32) -> torch.Tensor:
+    def vjp_a8(self, gy_codes, gy_scales, grad_input: Optional[torch.Tensor] = None, out_dtype=None) -> torch.Tensor:
         """grad_input = grad_output @ deq(W), overwriting it; grad_output as e4m3fn codes [M, OUT] with scales
-        [M, ceil(OUT/128)].  The layer must have been made with ``grad=True``."""
+        [M, ceil(OUT/128)].  The layer must have been made with ``grad=True``.  `out_dtype` (fp32 or bf16) as in
+        `forward_a8`, fp32 where neither it nor grad_input is given."""
         M = self._codes(gy_codes, gy_scales, self.OUT, "FP8BlockLinear.vjp_a8")
+        if out_dtype is None:
+            out_dtype = torch.float32 if grad_input is None else grad_input.dtype
         if out_dtype not in _TORCH_DT:
             raise L.NQError(L.NQ_ERR_INVALID, "FP8BlockLinear.vjp_a8: gx must be fp32 or bf16")
         if grad_input is None:
@@ -517,7 +524,7 @@ class FP8BlockLinear(_Layer):
         return grad_input
 
     def vjp(self, forward_input: Optional[torch.Tensor], grad_output: torch.Tensor,
-            grad_input: Optional[torch.Tensor] = None, out_dtype=torch.float32) -> torch.Tensor:
+            grad_input: Optional[torch.Tensor] = None, out_dtype=None) -> torch.Tensor:
         """`vjp_a8` of an fp32 or bf16 grad_output, quantised per row and block of 128 of OUT first (the gradient is
         linear in it and does not depend on forward_input, which may be None)."""
         if grad_output.dtype not in _TORCH_DT:

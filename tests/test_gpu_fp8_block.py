@@ -506,3 +506,30 @@ def test_recorded_into_graphs_and_on_two_streams():
         yb = [lin.forward(xs[0]) for _ in range(4)]
     torch.cuda.synchronize()
     assert all(torch.equal(t, lin.forward(xs[1])) for t in ya) and all(torch.equal(t, lin.forward(xs[0])) for t in yb)
+
+
+def test_output_types():
+    """y and gx are of `out_dtype`, of the given output's type without one, and bf16 / fp32 where neither is given."""
+    gen = torch.Generator().manual_seed(9)
+    wq, ws = R.random_weight(gen, 144, 272)
+    lin = layer(wq, ws, grad=True)
+    x, gy = torch.randn(5, 272, generator=gen).cuda(), torch.randn(5, 144, generator=gen).cuda()
+    codes, grads = quantize_rows_fp8_block(x), quantize_rows_fp8_block(gy)
+    for dtype in DTYPES:
+        y, gx = torch.empty((5, 144), dtype=dtype, device="cuda"), torch.empty((5, 272), dtype=dtype, device="cuda")
+        want, wantx = lin.forward_a8(*codes, out_dtype=dtype), lin.vjp_a8(*grads, out_dtype=dtype)
+        assert want.dtype == wantx.dtype == dtype
+        for call in (lambda: lin.forward_a8(*codes, out=y), lambda: lin.forward(x, out=y), lambda: lin.forward(x, out=y, out_dtype=dtype)):
+            y.fill_(7.0)
+            assert call() is y and torch.equal(y, want)
+        for call in (lambda: lin.vjp_a8(*grads, grad_input=gx), lambda: lin.vjp(None, gy, grad_input=gx),
+                     lambda: lin.vjp(None, gy, gx, out_dtype=dtype)):
+            gx.fill_(7.0)
+            assert call() is gx and torch.equal(gx, wantx)
+    assert lin.forward(x).dtype == torch.bfloat16 and lin.vjp(None, gy).dtype == torch.float32
+    with pytest.raises(NQError, match="out must be torch.float32"):
+        lin.forward_a8(*codes, out=y, out_dtype=torch.float32)
+    with pytest.raises(NQError, match="grad_input must be torch.float32"):
+        lin.vjp_a8(*grads, grad_input=gx, out_dtype=torch.float32)
+    with pytest.raises(NQError, match="fp32 or bf16"):
+        lin.forward_a8(*codes, out=y.half())
