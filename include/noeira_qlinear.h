@@ -280,7 +280,8 @@ int32_t nq_slice_cast_f32(const uint16_t* src, float* dst, int32_t rows, int32_t
  * row and block of 128 of K (the last one as wide as is left)
  *     s = absmax / 448 (1 where the block is zero, never below 2^-126);  q = e4m3(clip(x / s, -448, 448))
  * divisions as IEEE rounds them, codes to nearest, ties to even.  A block that holds a NaN or an infinity gets the scale
- * NaN and codes 0x7F: all its values are NaN.  x F32 or BF16, any K >= 1; x and codes 16-byte aligned. */
+ * NaN and codes 0x7F: all its values are NaN.  x F32 or BF16, any K >= 1; x and codes 16-byte aligned; what is read and
+ * what is written do not overlap. */
 int32_t nq_quantize_rows_fp8_block(const void* x, int32_t x_dtype, uint8_t* codes, float* scales, int32_t M, int32_t K,
                                    void* stream);
 
@@ -293,10 +294,11 @@ int32_t nq_grad_input_fp8_block(nq_handle h, const uint8_t* gy, const float* gy_
                                 int32_t M, void* stream);
 
 /* Layer norm over rows of D values, y[M, D] = (x - mean) * rstd * gamma + beta with rstd = 1 / sqrt(var + eps), the
- * variance divided by D; statistics in fp32.  x and y F32 or BF16 (y may be x where the types agree; otherwise they do
+ * variance divided by D; statistics in fp32 (a row whose centred squares overflow there has rstd 0, and with eps = 0 one
+ * whose variance is 0 there has rstd infinite: no call refuses it).  x and y F32 or BF16 (y may be x where the types agree; otherwise they do
  * not overlap); gamma, beta fp32 [D], or NULL for 1 and 0; mean, rstd fp32 [M] for the gradient, or both NULL.
  * The _fp8_block form writes y as nq_quantize_rows_fp8_block would (codes [M, D], scales [M, ceil(D/128)]) from the fp32
- * result, which is never stored: the norm in front of an FP8_BLOCK projection in one launch. */
+ * result, which is never stored: the norm in front of an FP8_BLOCK projection in one launch.  Its outputs overlap no input. */
 int32_t nq_layer_norm(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps, void* y,
                       int32_t y_dtype, float* mean, float* rstd, int32_t M, int32_t D, void* stream);
 int32_t nq_layer_norm_fp8_block(const void* x, int32_t x_dtype, const float* gamma, const float* beta, float eps,
@@ -305,8 +307,8 @@ int32_t nq_layer_norm_fp8_block(const void* x, int32_t x_dtype, const float* gam
 /* The gradients of nq_layer_norm from its input, its saved statistics and gy[M, D]:
  *     a = gy * gamma, xh = (x - mean) * rstd
  *     gx = rstd * (a - mean_D(a) - xh * mean_D(a * xh)),  dgamma = sum_M gy * xh,  dbeta = sum_M gy
- * gx [M, D] F32 or BF16 (gx may be gy, or x, where the types agree); dgamma, dbeta fp32 [D] are overwritten (zeros for
- * M = 0), or both NULL: no sums over the rows.  Their partial sums lie in `workspace` (16-byte aligned, at least
+ * gx [M, D] F32 or BF16 (gx may be gy, or x, where the types agree, and overlaps nothing otherwise); dgamma, dbeta
+ * fp32 [D] are overwritten (zeros for M = 0), or both NULL: no sums over the rows.  Their partial sums lie in `workspace` (16-byte aligned, at least
  * nq_layer_norm_grad_workspace_bytes(M, D); 0 where a few rows need none), which holds nothing between calls; two calls
  * that may run at once need one each.  The rows are added in a fixed order: the same inputs give the same bits.  D <= 2^26. */
 int64_t nq_layer_norm_grad_workspace_bytes(int32_t M, int32_t D);

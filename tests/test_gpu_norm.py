@@ -69,6 +69,50 @@ def test_forward_into_codes(M, D, dtype):
     assert torch.equal(again[0].view(torch.uint8), codes.view(torch.uint8)) and torch.equal(again[1], scales)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,D", [(8193, 7), (20000, 64), (9001, 1001), (2100, 1032), (2050, 2567), (2100, 4096), (1500, 4104), (1030, 8191),
+                                 (700, 8200), (530, 11007), (600, 16384)])
+def test_more_rows_than_teams(M, D, dtype):
+    """More rows than the chip holds teams of 64, 256, 512 and 1024 threads (8192, 2048, 1024 and 512): a team walks several,
+    the next one requested before the current one is done; y as values and as codes, in place too."""
+    norm, x, _ = inputs(M, D, dtype, 7)
+    y, mean, rstd, e_y, e_mean, r_rstd = R.norm(x, norm.gamma, norm.beta, EPS)
+    got, gm, gr = norm.forward_train(x)
+    R.assert_within(got, y, e_y + R.HALF_STEP[dtype] * (y.abs() + e_y), "y")
+    R.assert_within(gm, mean, e_mean, "mean")
+    R.assert_within(gr, rstd, rstd * r_rstd, "rstd")
+    codes, scales, cm, cr = norm.forward_fp8_train(x)
+    want = quantize_rows_fp8_block(norm.forward(x, out_dtype=torch.float32))
+    assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
+    assert torch.equal(cm, gm) and torch.equal(cr, gr)
+    z = x.clone()
+    norm.forward(z, out=z)
+    assert torch.equal(z, got)
+
+
+@pytest.mark.parametrize("D", [20, 960, 1001, 16391])
+def test_rows_at_the_ends_of_fp32(D):
+    """Statistics are fp32: a row whose squares overflow has rstd 0 and y = beta, one whose squares vanish has
+    rstd = 1 / sqrt(eps); without eps a row of one value has rstd infinite and y NaN, as the formula says, and its
+    neighbours keep their bits."""
+    norm, x, gen = inputs(4, D, torch.float32, 8)
+    sign = torch.where(torch.rand(D, generator=gen) < 0.5, -1.0, 1.0).cuda()
+    sign[:2] = torch.tensor([1.0, -1.0])
+    clean = norm.forward(x)
+    x[1], x[2] = 1e25 * sign, 1e-30 * sign
+    y, mean, rstd = norm.forward_train(x)
+    assert rstd[1] == 0 and torch.equal(y[1], norm.beta)
+    assert (rstd[2].double() * EPS ** 0.5 - 1).abs() <= 4 * R.U and (y[2] - norm.beta).abs().max() < 1e-24
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
+    codes, scales = norm.forward_fp8(x)
+    assert torch.isfinite(scales).all() and torch.equal(scales[1], quantize_rows_fp8_block(norm.beta.view(1, D))[1][0])
+    bare = LayerNorm(D, eps=0.0)
+    x[1] = 0.5
+    y, mean, rstd = bare.forward_train(x)
+    assert rstd[1] == float("inf") and torch.isnan(y[1]).all() and torch.isfinite(y[[0, 3]]).all()
+    assert torch.isnan(bare.forward_fp8(x)[1][1]).all() and torch.isfinite(bare.forward_fp8(x)[1][[0, 3]]).all()
+
+
 @pytest.mark.parametrize("D", [1, 129, 960, 4096, 16391])
 def test_constant_rows_and_far_means(D):
     """A row of one value has variance 0: y is beta exactly; a row far from zero loses what its mean's rounding costs, and
