@@ -148,7 +148,9 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_block_kernel(const void
 // in wavefront order (bit-repeatable).  U: blocks requested together.  Both operands go from memory to registers: the
 // weight's tiles are contiguous, every byte of them is read once per 16 MT rows, and at one row nothing else matters.
 // One row over 4096 -> 11008 (45 MB, rotating over copies): 9.1 us in bf16, 4.9 TB/s (a plain copy moves 5.0); 256 rows over
-// 4096 -> 4096: 15.2, 134 MB from L2 (11 TB/s, which bounds every call from about 16 rows on).
+// 4096 -> 4096: 15.2, 134 MB from L2 at 11 TB/s.  That is the rate of these loads, 64 bytes of a row of x at a time, and it
+// bounds the calls from about 16 rows on; it is not the path's: transfers into LDS reach 16 - 21 TB/s in the GEMMs of this
+// library.  (64 / 128 / 256 rows: 2.4 / 3.4 / 3.9 times the floor of their bytes and products.)
 template <int MT, int NT, int KW, int U, bool EXACT>
 __global__ __launch_bounds__(64 * KW) void fp8_block_tile_kernel(const BlockParams p) {
     constexpr int ROWS = 16 * MT, CH = 16 * NT;

@@ -17,8 +17,8 @@
 // 33 (their matrix core time).  The transfers cost what they occupy of LDS (64 KiB in, 192 KiB of fragments out per stage:
 // 2048 cycles at 128 B, as many as the products), the multiply-adds about half of their 1024 vector cycles per stage and
 // SIMD.  On 128 x 128 tiles LDS is the bound outright (128 KiB per 512 cycles of products: 0.47 us a stage; 18.2 - 20.6 us
-// a round at K = 4096).  With an fp32 y the two bf16 products per fp8 one and 16 conversions per fragment take 239 us
-// (1.15 PFLOP/s; a library bf16 product of the same size 232).
+// a round at K = 4096).  With an fp32 y the two bf16 products per fp8 one and 16 conversions per fragment take
+// 239 - 252 us (1.1 - 1.15 PFLOP/s; a library bf16 product of the same size 232).
 #include <algorithm>
 
 #include "nq_fp8_block.h"

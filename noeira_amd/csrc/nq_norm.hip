@@ -13,11 +13,11 @@
 // walked in passes (the *_long kernels).
 // Measured, 8192 x 4096 in bf16: y in bf16 24 us (134 MB, 5.6 TB/s, a copy's rate), codes 22.5 - 23.3 (102 MB, 4.4 TB/s: the
 // vector ALU, about 13 instructions a value, beside the two barriers a row); backward 38.3 + 4.8 (201 MB, 5.2 TB/s, and the
-// partials).  fp32 in and out: 42 us (6.4 TB/s).
+// partials).  fp32 in and out: 42 - 46 us (5.9 - 6.4 TB/s).
 //
 // 16 lanes hold 128 adjacent values: the block that shares a scale, so the quantised form needs one reduction over a DPP
 // row per vector and nothing else.  Rows whose length is no multiple of 8 are not 16-byte aligned: there a lane takes
-// every 16th value of its block instead of 8 adjacent ones, one load each (8192 x 4095 in bf16: 31.7 us).
+// every 16th value of its block instead of 8 adjacent ones, one load each (8192 x 4095 in bf16: 32 - 35 us).
 #include <algorithm>
 
 #include "nq_common.h"
@@ -224,7 +224,9 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const Nor
     }
 }
 
-// rows beyond 16384 values: one workgroup per row, three passes (the row comes from the caches after the first)
+// Rows beyond 16384 values: one workgroup per row, three passes (the row comes from the caches after the first), one value per
+// load.  1024 x 32768: 157 us in fp32 (1.7 TB/s), 125 in bf16 (1.1), 145 and 123 into codes; the gradient below 174 and 177.
+// Half the bytes take nearly the same time: the number of loads bounds it, not memory (54 and 27 us; 81 and 40).
 __global__ __launch_bounds__(1024) void layer_norm_long_kernel(const NormArgs a) {
     __shared__ float lds[2][16];
     const int wave = threadIdx.x / 64;
@@ -572,11 +574,12 @@ int32_t launch_norm(const NormArgs& a, hipStream_t s) {
 }
 
 // Where both gradients come from one launch and no partials (layer_norm_grad_once_kernel): its columns take a time that grows
-// with M / slices, and the rows are read twice.  Partials / one launch, us: 1 x 960 7.4 / 4.4 (a launch saved), 333 x 1001 fp32
-// 9.0 / 4.4, 1024 x 960 fp32 9.9 / 7.3, 2048 x 960 12.9 / 12.2, 512 x 4096 fp32 18.4 / 10.0, 1024 x 4096 fp32 20.6 / 18.3, 1536 x 4096
-// 25.7 / 27.4, 1024 x 8192 47.8 / 36.7, 1024 x 11008 51.9 / 54.4; rows of odd length, whose columns lie across lines: 512 x
-// 4095 15.6 / 12.0, 1024 x 4095 18.5 / 23.2, 333 x 8191 17.1 / 18.2, but 512 x 11007 39.4 / 36.2 (the other kernel's 16 values per
-// thread spill there).
+// with M / slices, and the rows are read twice.  Partials / one launch, us, in fp32 (bf16 in brackets): 1 x 960 7.4 / 4.4 (a
+// launch saved), 333 x 1001 9.0 / 4.4 (8.9 / 3.5), 1024 x 960 9.9 / 7.3 (8.6 / 6.8), 2048 x 960 13.2 / 12.6 (10.4 / 10.9), 512 x 4096
+// 18.4 / 10.0 (16.1 / 8.7), 1024 x 4096 20.6 / 18.3 (17.8 / 14.8), 1536 x 4096 25.7 / 27.4 (17.5 / 21.8), 1024 x 8192 47.8 / 36.7
+// (37.4 / 29.5), 1024 x 11008 51.9 / 54.4 (37.0 / 38.2); rows of odd length, whose columns lie across lines: 512 x 4095 15.6 / 12.0
+// (14.5 / 10.2), 1024 x 4095 18.5 / 23.2 (17.4 / 18.7), 333 x 8191 17.1 / 18.2 (18.5 / 17.8), but 512 x 11007 39.4 / 36.2 (37.1 /
+// 29.9; the other kernel's 16 values per thread need 84 bytes of scratch memory there).
 bool grad_once(int32_t M, int32_t D) {
     return D <= MAX_HELD && M <= 1024 && (int64_t)M * D <= (D % 8 == 0 || D > 8192 ? 1 << 23 : 1 << 21);
 }
