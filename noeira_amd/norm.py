@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
-from .qlinear import _FLOATS, _TORCH_DT, _check_dev, _check_int32, _dev_ptr, _need_gpu, _stream_now
+from .qlinear import _FLOATS, _INT32_MAX, _TORCH_DT, _check_dev, _dev_ptr, _need_gpu, _stream_now, _too_many
 
 
 class LayerNorm:
@@ -22,7 +22,8 @@ class LayerNorm:
     def __init__(self, DIM: int, eps: float = 1e-5):
         if DIM < 1:
             raise L.NQError(L.NQ_ERR_INVALID, "LayerNorm: DIM must be positive")
-        _check_int32(DIM, "LayerNorm", "values in a row")
+        if DIM > _INT32_MAX:
+            raise _too_many(DIM, "LayerNorm", "values in a row")
         self.DIM, self.eps = int(DIM), float(eps)
         self.gamma = torch.ones((DIM,), dtype=torch.float32, device="cuda")
         self.beta = torch.zeros((DIM,), dtype=torch.float32, device="cuda")
@@ -50,7 +51,8 @@ class LayerNorm:
         M = x.numel() // self.DIM
         if M * self.DIM != x.numel():
             raise L.NQError(L.NQ_ERR_INVALID, f"{what}: x has {x.numel()} values, not a multiple of DIM = {self.DIM}")
-        _check_int32(M, what, "rows")
+        if M > _INT32_MAX:
+            raise _too_many(M, what, "rows")
         return M
 
     def _like(self, x: torch.Tensor, M: int, dtype: torch.dtype) -> torch.Tensor:

@@ -75,10 +75,12 @@ def _check_dev(t: torch.Tensor, who: str, name: str, dtype=None, numel=None):
     return t
 
 
-def _check_int32(n: int, what: str, name: str):
-    """The C ABI counts rows and columns in 32 bits, and ctypes would cut a longer count without a word."""
-    if n > 0x7FFFFFFF:
-        raise L.NQError(L.NQ_ERR_SIZE, f"{what}: {n} {name}, at most 2^31 - 1 in a call")
+# The C ABI counts rows and columns in 32 bits, and ctypes would cut a longer count without a word.
+_INT32_MAX = 0x7FFFFFFF
+
+
+def _too_many(n: int, what: str, name: str) -> L.NQError:
+    return L.NQError(L.NQ_ERR_SIZE, f"{what}: {n} {name}, at most 2^31 - 1 in a call")
 
 
 def _check_x(x: torch.Tensor, IN: int, what: str):
@@ -468,7 +470,8 @@ class FP8BlockLinear(_Layer):
         M = codes.numel() // K
         if M * K != codes.numel():
             raise L.NQError(L.NQ_ERR_INVALID, f"{what}: the codes are {codes.numel()} values, not a multiple of {K}")
-        _check_int32(M, what, "rows")
+        if M > _INT32_MAX:
+            raise _too_many(M, what, "rows")
         _check_dev(scales, what, "the scales", torch.float32, M * (-(-K // 128)))
         return M
 
@@ -733,8 +736,8 @@ def quantize_rows_fp8_block(x: torch.Tensor, codes: Optional[torch.Tensor] = Non
         raise L.NQError(L.NQ_ERR_INVALID, "quantize_rows_fp8_block: x must be a contiguous fp32/bf16 [M, K] device tensor")
     _check_dev(x, "quantize_rows_fp8_block", "x")
     M, K = x.shape
-    _check_int32(M, "quantize_rows_fp8_block", "rows")
-    _check_int32(K, "quantize_rows_fp8_block", "columns")
+    if M > _INT32_MAX or K > _INT32_MAX:
+        raise _too_many(max(M, K), "quantize_rows_fp8_block", "rows" if M > K else "columns")
     G = -(-K // 128)
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
